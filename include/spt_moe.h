@@ -112,6 +112,59 @@ typedef struct spt_moe_taps {
     float *results;         /* [B*k][H] down projection + bias               */
 } spt_moe_taps;
 
+/* A quantized key/value cache: n_pages pages of page_len positions, each
+ * position n_kv_heads keys and values of head_dim elements in GGML blocks of
+ * 32 (Q4_0: 18 bytes a block, 144 KB for 1,024 positions of 8 heads of 64;
+ * Q8_0: 34).  The order of the bytes in a page is the library's own (a page
+ * is copied whole); spt_kv_load_batch reads positions back.  head_dim is 64
+ * or 128, page_len a multiple of 32.  Replaces forward.KVCache
+ * (forward/attention.go:11, fp32, one sequence of 2,048 positions). */
+typedef struct spt_kv_cache {
+    uint32_t type; /* SPT_TYPE_Q4_0 or SPT_TYPE_Q8_0, keys and values        */
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    int32_t page_len;
+    int64_t n_pages;
+    uint64_t nbytes; /* spt_kv_cache_bytes                                   */
+    void *data;      /* device address, 16-byte aligned; need not be cleared */
+} spt_kv_cache;
+
+/* The sequences of a call.  Row buffers (q, k, v, out) hold n_rows rows of
+ * heads; sequence s has rows [rows_dev[s], rows_dev[s+1]), which are its last
+ * positions: it is lens_dev[s] positions long with them, and its position p is
+ * in page pages_dev[s * max_pages + p / page_len].  rows_dev, lens_dev and
+ * pages_dev are device memory, read by the kernels (a captured graph may be
+ * replayed with other lengths and pages in them); the other fields bound them.
+ * What they say is not trusted: rows outside the buffers are left out; a row of
+ * a position before the first (more rows than positions) is not stored, loads
+ * as NaN and attends to nothing; a page outside [0, n_pages) is not stored to,
+ * loads as NaN and gives NaN to whoever attends to it; a sequence of more than
+ * max_new rows or longer than max_len is not stored, and its first max_new
+ * rows load and attend as NaN (its others are left as they were).  Rows
+ * that belong to no sequence are left as they were.  No two sequences of a
+ * store may share a page that it writes, and no two rows a position. */
+typedef struct spt_kv_batch {
+    int32_t n_seqs;    /* at most 65,535                                     */
+    int32_t max_new;   /* most rows of a sequence                            */
+    int64_t n_rows;
+    int64_t max_len;   /* longest sequence (at most 2^30 and max_pages * page_len) */
+    int32_t max_pages; /* row length of pages_dev                            */
+    const int32_t *rows_dev;  /* [n_seqs + 1]                                */
+    const int32_t *lens_dev;  /* [n_seqs]                                    */
+    const int32_t *pages_dev; /* [n_seqs][max_pages]                         */
+} spt_kv_batch;
+
+/* Rotary embedding of pairs (i, i + head_dim/2) with the YaRN ramp
+ * (forward/rope.go:15-52): factor 1 is plain rotation, and then the last
+ * three fields are not read.  GPT-OSS: 150000, 32, 4096, 32, 1. */
+typedef struct spt_rope {
+    float base;
+    float factor;
+    int32_t original_len;
+    float beta_fast;
+    float beta_slow;
+} spt_rope;
+
 /* ---- context ----------------------------------------------------------- */
 
 /* Thread-local message of the last failed call on this thread. */
@@ -164,7 +217,9 @@ enum {
     SPT_KERNEL_DOWN_GEMM = 8,    /* grouped down GEMM (large groups)          */
     SPT_KERNEL_Q80 = 9,      /* Q8_0 LM head (GEMV or argmax)                 */
     SPT_KERNEL_RMSNORM = 10, /* RMSNorm (+ Q8_0 of its output)                */
-    SPT_KERNEL_KINDS = 11
+    SPT_KERNEL_KV = 11,      /* key/value cache store and load                */
+    SPT_KERNEL_ATTENTION = 12, /* attention over the cache                    */
+    SPT_KERNEL_KINDS = 13
 };
 int spt_ctx_enable_timing(struct spt_ctx *ctx, int enable);
 /* Synchronise, then write the summed milliseconds and launch counts of each
@@ -307,6 +362,61 @@ int spt_rmsnorm_into(struct spt_ctx *ctx, const spt_tensor *weight, const float 
 int spt_rmsnorm_batch_into(struct spt_ctx *ctx, const spt_tensor *weight, const float *x_dev,
                            int64_t x_len, float *y_dev, int64_t y_len, int64_t batch, float epsilon,
                            void *q8_dev);
+
+/* ---- key/value cache and attention -------------------------------------- */
+
+/* Bytes of a cache (spt_kv_cache.nbytes). */
+int spt_kv_cache_bytes(uint32_t type, int32_t n_kv_heads, int32_t head_dim, int32_t page_len,
+                       int64_t n_pages, uint64_t *out);
+
+/* ApplyRoPE on queries and keys (forward/rope.go:15) and the write of keys and
+ * values into the cache (forward/attention.go:11-57), in one launch: q_out =
+ * rot(q), and the rows' positions of the cache = Q(rot(k)), Q(v).  rope NULL:
+ * keys are stored as they are, and there are no queries.  q_dev NULL (and
+ * q_out_dev, lengths 0): no queries; q_out may be q.  Rows are
+ * [n_rows][heads][head_dim] fp32, 16-byte aligned; heads of q any multiple of
+ * n_kv_heads.  Angles, sines and products are taken in 64 bits and rounded once.
+ * Q is GGML's quantization in 32 bits (Q4_0: d = m / -8, m the first element of
+ * the largest magnitude, code min(15, floor(x * (1/d) + 8.5)); Q8_0 as
+ * spt_quantize_q8_0), with |d| at most 8188 (Q4_0) and 515.5 (Q8_0): larger
+ * values saturate at about 65,504.  An infinity or NaN anywhere in a row's key
+ * or value of a head makes that key NaN and that value 0, so that
+ * attention to it gives NaN. */
+int spt_kv_store_batch(struct spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch,
+                       const spt_rope *rope, const float *q_dev, int64_t q_len, float *q_out_dev,
+                       int64_t q_out_len, const float *k_dev, int64_t k_len, const float *v_dev,
+                       int64_t v_len);
+
+/* The cache read back: the batch's rows' positions as fp32 keys and values
+ * (code * d, exact), [n_rows][n_kv_heads][head_dim].  To read a sequence from
+ * its start, give it as many rows as positions.  No reference counterpart (its
+ * cache is fp32). */
+int spt_kv_load_batch(struct spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch,
+                      float *k_dev, int64_t k_len, float *v_dev, int64_t v_len);
+
+/* forwardAttention (forward/attention.go:59-160) of the batch's rows, whose
+ * keys and values are in the cache already: out = sum_j p_j v_j / (sum_j p_j +
+ * exp(sink - top)), p_j = exp(scale * q . k_j - top) over positions j up to the
+ * row's own and, with window > 0, fewer than window before it.  sinks: optional
+ * F32 / F16 / BF16 [heads]; NULL or unnamed: none.  A row that sees nothing is 0.
+ * Scores, sums and outputs are at fp32's accuracy.  q8_dev: NULL, or
+ * q_len/32 GGML Q8_0 blocks that receive the Q8_0 of out, the input of
+ * spt_mul_q40_batch_q8_into.  out must not overlap q.
+ * work_dev: a workspace of spt_attention_work_bytes bytes, 16-byte aligned, or
+ * NULL: the context's arena.  With a workspace the call allocates nothing, so
+ * it may be captured into a graph; give each graph and each stream its own.
+ * Results do not depend on which is used, nor change from call to call. */
+int spt_attention_batch_into(struct spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch,
+                             const spt_tensor *sinks, float scale, int32_t window, const float *q_dev,
+                             int64_t q_len, float *out_dev, int64_t out_len, void *q8_dev,
+                             void *work_dev, uint64_t work_bytes);
+
+/* The workspace of an attention call on this cache and a batch of these sizes
+ * (0: none needed). */
+int spt_attention_work_bytes(struct spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch,
+                             int32_t n_heads, int32_t window, uint64_t *out);
+
+/* ---- mixture of experts --------------------------------------------------- */
 
 /* forward.mulMoEBatchExpert (forward/mxfp4_batch.go:29-53) for one expert of
  * an MXFP4 [in, out, experts] tensor with consecutive (not gathered) rows:

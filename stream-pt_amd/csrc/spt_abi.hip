@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <cerrno>
 #include <climits>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -17,6 +18,7 @@
 #include <vector>
 
 #include "spt_kernels.h"
+#include "spt_kv.h"
 #include "spt_moe.h"
 
 struct spt_ctx {
@@ -1199,6 +1201,123 @@ int load_range(spt_ctx *ctx, const std::string &path, uint64_t start, uint64_t n
     return rc;
 }
 
+// ---- the key/value cache and attention over it
+
+int kv_type_bits(uint32_t type) { return type == SPT_TYPE_Q4_0 ? 4 : type == SPT_TYPE_Q8_0 ? 8 : 0; }
+
+constexpr int64_t kKvMaxLen = int64_t(1) << 30;  // positions of a sequence
+
+int kv_cache_size(uint32_t type, int64_t kv_heads, int64_t head_dim, int64_t page_len, int64_t n_pages, uint64_t *out) {
+    if (!kv_type_bits(type))
+        return fail(SPT_ERR_INVALID, "key/value cache: GGML type %u instead of Q4_0 (2) or Q8_0 (8)", type);
+    if (head_dim != 64 && head_dim != 128)
+        return fail(SPT_ERR_INVALID, "key/value cache: head dimension %lld is not 64 or 128", (long long)head_dim);
+    if (page_len <= 0 || page_len % spt::kKvTile != 0 || page_len > kKvMaxLen)
+        return fail(SPT_ERR_INVALID, "key/value cache: page length %lld is not a multiple of %d", (long long)page_len, spt::kKvTile);
+    int64_t n;
+    if (kv_heads > 65535 || n_pages > INT_MAX ||
+        !product(&n, {n_pages, kv_heads, page_len / spt::kKvTile, spt::kv_tile_bytes(kv_type_bits(type), (int)head_dim / 32)}))
+        return fail(SPT_ERR_INVALID, "key/value cache: invalid shape of %lld pages and %lld heads", (long long)n_pages, (long long)kv_heads);
+    *out = (uint64_t)n;
+    return SPT_OK;
+}
+
+int kv_check(const spt_kv_cache *c, const spt_kv_batch *b, int *bits, int *nb, spt::KvArgs *a) {
+    if (!c || !b) return fail(SPT_ERR_INVALID, "nil key/value cache or batch");
+    uint64_t bytes;
+    int rc;
+    if ((rc = kv_cache_size(c->type, c->n_kv_heads, c->head_dim, c->page_len, c->n_pages, &bytes))) return rc;
+    if (c->nbytes != bytes)
+        return fail(SPT_ERR_INVALID, "key/value cache: %llu bytes instead of %llu", (unsigned long long)c->nbytes, (unsigned long long)bytes);
+    if (!c->data || ((uintptr_t)c->data & 15)) return fail(SPT_ERR_INVALID, "key/value cache: data must be resident and 16-byte aligned");
+    if (b->n_seqs < 0 || b->n_seqs > 65535 || b->n_rows < 0 || b->n_rows > INT_MAX || b->max_new < 1 || b->max_len < 1 ||
+        b->max_len > kKvMaxLen || b->max_pages < 1)
+        return fail(SPT_ERR_INVALID, "key/value batch: invalid sizes (%d sequences, %lld rows, at most %d new, %lld long, %d pages)", b->n_seqs,
+                    (long long)b->n_rows, b->max_new, (long long)b->max_len, b->max_pages);
+    if (b->max_len > (int64_t)b->max_pages * c->page_len)
+        return fail(SPT_ERR_INVALID, "key/value batch: %lld positions do not fit %d pages of %d", (long long)b->max_len, b->max_pages, c->page_len);
+    if (!b->rows_dev || !b->lens_dev || !b->pages_dev || (((uintptr_t)b->rows_dev | (uintptr_t)b->lens_dev | (uintptr_t)b->pages_dev) & 3))
+        return fail(SPT_ERR_INVALID, "key/value batch: nil or unaligned rows, lengths or pages");
+    *bits = kv_type_bits(c->type);
+    *nb = c->head_dim / 32;
+    *a = spt::KvArgs{(uint8_t *)c->data, c->n_kv_heads, c->page_len / spt::kKvTile, c->n_pages, b->n_seqs, b->max_new, (int)b->n_rows,
+                     (int)b->max_len, b->max_pages, b->rows_dev, b->lens_dev, b->pages_dev};
+    return SPT_OK;
+}
+
+// A buffer of n_rows rows of heads: its length, address and place apart from the cache.
+int kv_rows_check(const char *what, const float *p, int64_t len, int64_t heads, const spt_kv_cache *c, const spt_kv_batch *b) {
+    if (heads <= 0 || heads > INT_MAX / c->head_dim || len / c->head_dim / heads != b->n_rows || len % (heads * c->head_dim) != 0)
+        return fail(SPT_ERR_INVALID, "%s: %lld elements do not hold %lld rows of %lld heads of %d", what, (long long)len, (long long)b->n_rows,
+                    (long long)heads, c->head_dim);
+    if (len && (!p || ((uintptr_t)p & 15))) return fail(SPT_ERR_INVALID, "%s: nil or not 16-byte aligned", what);
+    if (ranges_overlap(p, (uint64_t)len * 4, c->data, c->nbytes)) return fail(SPT_ERR_INVALID, "%s overlaps the key/value cache", what);
+    return SPT_OK;
+}
+
+// Query heads of a buffer of len elements.
+int kv_query_heads(int64_t len, const spt_kv_cache *c, const spt_kv_batch *b, int64_t *heads) {
+    *heads = b->n_rows ? len / b->n_rows / c->head_dim : c->n_kv_heads;
+    if (*heads < c->n_kv_heads || *heads % c->n_kv_heads != 0 || *heads > 65535)
+        return fail(SPT_ERR_INVALID, "queries: %lld elements in %lld rows are not a multiple of %d heads of %d", (long long)len,
+                    (long long)b->n_rows, c->n_kv_heads, c->head_dim);
+    return SPT_OK;
+}
+
+// Rotary frequencies with the YaRN ramp: pair i turns base^(-2i/dim) a
+// position; pairs that turn less than `slow` times within the original length
+// are slowed by `factor`, those that turn more than `fast` times are not, the
+// ramp between them is linear in i; cos and sin are scaled by
+// 0.1 ln(factor) + 1 (forward/rope.go:15-52).
+int rope_table(const spt_rope *r, int dim, spt::RopeTable *t) {
+    const double base = r->base, factor = r->factor, fast = r->beta_fast, slow = r->beta_slow;
+    const bool ramp = factor > 1.0;
+    if (!(base > 1.0) || !(factor >= 1.0) || !std::isfinite(base) || !std::isfinite(factor) ||
+        (ramp && (!(slow > 0.0) || !(fast > slow) || !std::isfinite(fast) || r->original_len < 1)))
+        return fail(SPT_ERR_INVALID, "invalid rotary embedding: base %g, factor %g, original length %d, betas %g and %g", base, factor,
+                    r->original_len, fast, slow);
+    const int h = dim / 2;
+    const double two_pi = 6.283185307179586477;
+    const double lo = ramp ? h * std::log(r->original_len / (fast * two_pi)) / std::log(base) : 0.0;
+    const double hi = ramp ? h * std::log(r->original_len / (slow * two_pi)) / std::log(base) : 1.0;
+    for (int i = 0; i < h; i++) {
+        const double f = std::pow(base, (double)i / h);
+        const double keep = ramp ? 1.0 - std::min(1.0, std::max(0.0, (i - lo) / (hi - lo))) : 1.0;
+        t->freq[i] = (1.0 - keep) / (factor * f) + keep / f;
+    }
+    t->mscale = 0.1 * std::log(factor) + 1.0;
+    return SPT_OK;
+}
+
+struct AttnCall {
+    int bits, nb;
+    spt::AttnArgs a;
+    uint64_t work_bytes;
+};
+
+// What attention launches for a batch, and the workspace that takes.
+int attn_setup(spt_ctx *ctx, const spt_kv_cache *c, const spt_kv_batch *b, int64_t heads, int32_t window, AttnCall *call) {
+    int rc;
+    if ((rc = kv_check(c, b, &call->bits, &call->nb, &call->a.kv))) return rc;
+    if (heads < c->n_kv_heads || heads % c->n_kv_heads != 0 || heads > 65535)
+        return fail(SPT_ERR_INVALID, "attention: %lld query heads are not a multiple of %d key/value heads", (long long)heads, c->n_kv_heads);
+    if (window < 0) return fail(SPT_ERR_INVALID, "attention: invalid window %d", window);
+    call->a.heads = (int)heads;
+    call->a.group = (int)(heads / c->n_kv_heads);
+    call->a.window = window >= b->max_len ? 0 : window;
+    if ((int64_t)b->max_new * call->a.group > INT_MAX / 2) return fail(SPT_ERR_INVALID, "attention: %d new rows are too many for one call", b->max_new);
+    const spt::AttnPlan p = spt::attn_plan(call->nb, c->n_kv_heads, call->a.group, std::max(1, b->n_seqs), b->max_new, (int)b->max_len,
+                                           call->a.window, ctx->n_cu > 0 ? ctx->n_cu : 256);
+    // a launch holds fewer than 2^32 threads
+    if ((int64_t)p.row_tiles * c->n_kv_heads * p.splits >= (int64_t(1) << 24))
+        return fail(SPT_ERR_INVALID, "attention: %d new rows are too many for one call", b->max_new);
+    call->a.row_tiles = p.row_tiles;
+    call->a.splits = p.splits;
+    call->a.split_tiles = p.split_tiles;
+    call->work_bytes = p.work_bytes;
+    return SPT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1647,6 +1766,127 @@ int spt_rmsnorm_batch_into(spt_ctx *ctx, const spt_tensor *weight, const float *
     if ((rc = check_device(ctx))) return rc;
     spt::RmsArgs a{x_dev, weight->data, wtype, (int)dim, (int)batch, epsilon, y_dev, (uint8_t *)q8_dev};
     SPT_HIP(timed(ctx, SPT_KERNEL_RMSNORM, [&] { return spt::launch_rmsnorm(ctx->stream, a, true); }));
+    return SPT_OK;
+}
+
+int spt_kv_cache_bytes(uint32_t type, int32_t n_kv_heads, int32_t head_dim, int32_t page_len, int64_t n_pages, uint64_t *out) {
+    if (!out) return fail(SPT_ERR_INVALID, "nil output pointer");
+    *out = 0;
+    return kv_cache_size(type, n_kv_heads, head_dim, page_len, n_pages, out);
+}
+
+int spt_kv_store_batch(spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch, const spt_rope *rope, const float *q_dev,
+                       int64_t q_len, float *q_out_dev, int64_t q_out_len, const float *k_dev, int64_t k_len, const float *v_dev,
+                       int64_t v_len) {
+    int rc, bits, nb;
+    if ((rc = check_ctx(ctx))) return rc;
+    spt::KvStoreArgs a{};
+    spt::RopeTable table{};
+    if ((rc = kv_check(cache, batch, &bits, &nb, &a.kv))) return rc;
+    if ((rc = kv_rows_check("keys", k_dev, k_len, cache->n_kv_heads, cache, batch))) return rc;
+    if ((rc = kv_rows_check("values", v_dev, v_len, cache->n_kv_heads, cache, batch))) return rc;
+    if (rope && (rc = rope_table(rope, cache->head_dim, &table))) return rc;
+    if (q_dev || q_out_dev || q_len || q_out_len) {
+        int64_t heads;
+        if (!rope) return fail(SPT_ERR_INVALID, "queries without a rotary embedding: there is nothing to do for them");
+        if (q_out_len != q_len) return fail(SPT_ERR_INVALID, "queries: %lld elements in and %lld out", (long long)q_len, (long long)q_out_len);
+        if ((rc = kv_query_heads(q_len, cache, batch, &heads))) return rc;
+        if ((rc = kv_rows_check("queries", q_dev, q_len, heads, cache, batch))) return rc;
+        if ((rc = kv_rows_check("rotated queries", q_out_dev, q_len, heads, cache, batch))) return rc;
+        const uint64_t qb = (uint64_t)q_len * 4;
+        if ((q_dev != q_out_dev && ranges_overlap(q_dev, qb, q_out_dev, qb)) || ranges_overlap(q_out_dev, qb, k_dev, (uint64_t)k_len * 4) ||
+            ranges_overlap(q_out_dev, qb, v_dev, (uint64_t)v_len * 4))
+            return fail(SPT_ERR_INVALID, "rotated queries partially overlap an input");
+        a.heads = (int)heads;
+    }
+    if ((rc = check_device(ctx)) || (rc = check_cancel(ctx))) return rc;
+    if (batch->n_seqs == 0 || batch->n_rows == 0) return SPT_OK;
+    a.k = k_dev;
+    a.v = v_dev;
+    a.q = q_dev;
+    a.q_out = q_out_dev;
+    a.rotate = rope != nullptr;
+    a.parts = spt::kv_store_parts(a.kv, ctx->n_cu);
+    SPT_HIP(timed(ctx, SPT_KERNEL_KV, [&] { return spt::launch_kv_store(ctx->stream, bits, nb, a, table); }));
+    return SPT_OK;
+}
+
+int spt_kv_load_batch(spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch, float *k_dev, int64_t k_len, float *v_dev,
+                      int64_t v_len) {
+    int rc, bits, nb;
+    if ((rc = check_ctx(ctx))) return rc;
+    spt::KvLoadArgs a{};
+    if ((rc = kv_check(cache, batch, &bits, &nb, &a.kv))) return rc;
+    if ((rc = kv_rows_check("keys", k_dev, k_len, cache->n_kv_heads, cache, batch))) return rc;
+    if ((rc = kv_rows_check("values", v_dev, v_len, cache->n_kv_heads, cache, batch))) return rc;
+    if (ranges_overlap(k_dev, (uint64_t)k_len * 4, v_dev, (uint64_t)v_len * 4)) return fail(SPT_ERR_INVALID, "keys and values overlap");
+    if ((rc = check_device(ctx)) || (rc = check_cancel(ctx))) return rc;
+    if (batch->n_seqs == 0 || batch->n_rows == 0) return SPT_OK;
+    a.k = k_dev;
+    a.v = v_dev;
+    SPT_HIP(timed(ctx, SPT_KERNEL_KV, [&] { return spt::launch_kv_load(ctx->stream, bits, nb, a); }));
+    return SPT_OK;
+}
+
+int spt_attention_work_bytes(spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch, int32_t n_heads, int32_t window,
+                             uint64_t *out) {
+    int rc;
+    if ((rc = check_ctx(ctx))) return rc;
+    if (!out) return fail(SPT_ERR_INVALID, "nil output pointer");
+    *out = 0;
+    AttnCall call{};
+    if ((rc = attn_setup(ctx, cache, batch, n_heads, window, &call))) return rc;
+    *out = call.work_bytes;
+    return SPT_OK;
+}
+
+int spt_attention_batch_into(spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch, const spt_tensor *sinks, float scale,
+                             int32_t window, const float *q_dev, int64_t q_len, float *out_dev, int64_t out_len, void *q8_dev,
+                             void *work_dev, uint64_t work_bytes) {
+    int rc;
+    if ((rc = check_ctx(ctx))) return rc;
+    if (!cache || !batch) return fail(SPT_ERR_INVALID, "nil key/value cache or batch");
+    AttnCall call{};
+    int64_t heads = 0;
+    if ((rc = kv_check(cache, batch, &call.bits, &call.nb, &call.a.kv))) return rc;
+    if ((rc = kv_query_heads(q_len, cache, batch, &heads))) return rc;
+    if ((rc = attn_setup(ctx, cache, batch, heads, window, &call))) return rc;
+    if (out_len != q_len) return fail(SPT_ERR_INVALID, "attention: %lld elements of queries and %lld of output", (long long)q_len, (long long)out_len);
+    if ((rc = kv_rows_check("queries", q_dev, q_len, heads, cache, batch))) return rc;
+    if ((rc = kv_rows_check("attention output", out_dev, out_len, heads, cache, batch))) return rc;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(SPT_ERR_INVALID, "attention: invalid scale %g", (double)scale);
+    const spt_tensor none{};
+    const spt_tensor &sk = sinks ? *sinks : none;
+    if ((rc = validate_bias(&sk, heads, 1))) return rc;
+    if (!elements_aligned(sk)) return fail(SPT_ERR_INVALID, "\"%s\": data must be aligned to its elements", tname(&sk));
+    const uint64_t qb = (uint64_t)q_len * 4, q8b = q8_dev ? (uint64_t)q_len / 32 * 34 : 0;
+    if (ranges_overlap(q_dev, qb, out_dev, qb)) return fail(SPT_ERR_INVALID, "attention: queries and output overlap");
+    if (ranges_overlap(q8_dev, q8b, q_dev, qb) || ranges_overlap(q8_dev, q8b, out_dev, qb) || ranges_overlap(q8_dev, q8b, cache->data, cache->nbytes))
+        return fail(SPT_ERR_INVALID, "attention: Q8_0 output overlaps the queries, the output or the cache");
+    if (work_dev) {
+        if (((uintptr_t)work_dev & 15) || work_bytes < call.work_bytes)
+            return fail(SPT_ERR_INVALID, "attention: the workspace must be 16-byte aligned and hold %llu bytes, got %llu",
+                        (unsigned long long)call.work_bytes, (unsigned long long)work_bytes);
+        if (ranges_overlap(work_dev, call.work_bytes, q_dev, qb) || ranges_overlap(work_dev, call.work_bytes, out_dev, qb) ||
+            ranges_overlap(work_dev, call.work_bytes, q8_dev, q8b) || ranges_overlap(work_dev, call.work_bytes, cache->data, cache->nbytes))
+            return fail(SPT_ERR_INVALID, "attention: the workspace overlaps an input or output");
+    }
+    if ((rc = check_device(ctx)) || (rc = check_cancel(ctx))) return rc;
+    if (batch->n_seqs == 0 || batch->n_rows == 0) return SPT_OK;
+    char *work = static_cast<char *>(work_dev);
+    if (!work && call.work_bytes && (rc = arena(ctx, call.work_bytes, &work))) return rc;
+    call.a.q = q_dev;
+    call.a.out = out_dev;
+    call.a.q8 = (uint8_t *)q8_dev;
+    call.a.sinks = bias_ptr(sk);
+    call.a.sink_type = bias_type(sk);
+    call.a.scale = scale * 1.44269504088896341f;
+    call.a.part = (float *)work;
+    SPT_HIP(timed(ctx, SPT_KERNEL_ATTENTION, [&] { return spt::launch_attn(ctx->stream, call.bits, call.nb, call.a); }));
+    if (call.a.splits > 1) {
+        if ((rc = check_cancel(ctx))) return rc;
+        SPT_HIP(timed(ctx, SPT_KERNEL_ATTENTION, [&] { return spt::launch_attn_merge(ctx->stream, call.nb, call.a); }));
+    }
     return SPT_OK;
 }
 

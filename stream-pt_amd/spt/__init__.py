@@ -12,7 +12,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 
-__all__ = ["SptError", "Tensor", "MoEConfig", "MoELayer", "MoETaps", "Context", "lib", "LIB_PATH",
+__all__ = ["SptError", "Tensor", "MoEConfig", "MoELayer", "MoETaps", "KVCache", "KVBatch", "Rope", "Context", "lib", "LIB_PATH",
            "TYPE_F32", "TYPE_F16", "TYPE_Q4_0", "TYPE_Q8_0", "TYPE_BF16", "TYPE_MXFP4",
            "OK", "ERR_INVALID", "ERR_DEVICE", "ERR_NOMEM", "ERR_CANCELED", "ERR_IO"]
 
@@ -34,9 +34,10 @@ EXPORTED = (
     "spt_rmsnorm_into", "spt_rmsnorm_batch_into", "spt_mul_q40_batch_bias_into",
     "spt_mul_q40_batch_q8_into", "spt_mul_q40_qkv_batch_into", "spt_forward_moe_batch_q8",
     "spt_forward_moe_batch_noalloc", "spt_ctx_set_decode_max_selections", "spt_upload_range", "spt_ctx_memory",
+    "spt_kv_cache_bytes", "spt_kv_store_batch", "spt_kv_load_batch", "spt_attention_batch_into", "spt_attention_work_bytes",
 )
 KERNEL_KINDS = ("quantize", "route", "gate_up", "down", "combine", "q40", "select", "gate_up_gemm", "down_gemm",
-                "q80", "rmsnorm")
+                "q80", "rmsnorm", "kv", "attention")
 
 
 class SptError(RuntimeError):
@@ -83,6 +84,57 @@ class MoETaps(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in (
         "logits_in", "logits", "ids", "weights", "counts", "offsets", "list", "active",
         "n_active", "xq", "gate", "up", "act", "actq", "results")]
+
+
+class KVCache(C.Structure):
+    """spt_kv_cache: pages of quantized keys and values in device memory."""
+    _fields_ = [("type", C.c_uint32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_len", C.c_int32),
+                ("n_pages", C.c_int64), ("nbytes", C.c_uint64), ("data", C.c_void_p)]
+
+    @staticmethod
+    def bytes(typ, kv_heads, head_dim, page_len, n_pages) -> int:
+        out = C.c_uint64()
+        _check(lib().spt_kv_cache_bytes(typ, kv_heads, head_dim, page_len, n_pages, C.byref(out)))
+        return out.value
+
+    @classmethod
+    def make(cls, typ, kv_heads, head_dim, page_len, n_pages, data):
+        """data: the device buffer (a tensor of cls.bytes(..) bytes, kept
+        on the descriptor, or an address)."""
+        n = cls.bytes(typ, kv_heads, head_dim, page_len, n_pages)
+        if hasattr(data, "element_size") and data.numel() * data.element_size() < n:
+            raise ValueError(f"a key/value cache of {n} bytes does not fit the buffer")
+        c = cls(typ, kv_heads, head_dim, page_len, n_pages, n, _ptr(data))
+        c._keep = data
+        return c
+
+
+class KVBatch(C.Structure):
+    """spt_kv_batch: the sequences of a call; the arrays are int32 device
+    tensors, kept on the descriptor."""
+    _fields_ = [("n_seqs", C.c_int32), ("max_new", C.c_int32), ("n_rows", C.c_int64), ("max_len", C.c_int64),
+                ("max_pages", C.c_int32), ("rows_dev", C.c_void_p), ("lens_dev", C.c_void_p), ("pages_dev", C.c_void_p)]
+
+    @classmethod
+    def make(cls, rows, lens, pages, n_rows, max_new, max_len):
+        """rows [n_seqs + 1], lens [n_seqs], pages [n_seqs][max_pages]."""
+        for t in (rows, lens, pages):
+            if t.element_size() != 4 or not t.is_contiguous():
+                raise ValueError("rows, lens and pages are contiguous int32 tensors")
+        if rows.numel() != lens.numel() + 1 or pages.dim() != 2 or pages.shape[0] != lens.numel():
+            raise ValueError("rows, lens and pages are of different numbers of sequences")
+        b = cls(lens.numel(), max_new, n_rows, max_len, pages.shape[1], _ptr(rows), _ptr(lens), _ptr(pages))
+        b._keep = (rows, lens, pages)
+        return b
+
+
+class Rope(C.Structure):
+    """spt_rope: Rope(base, factor=1, original_len, beta_fast, beta_slow)."""
+    _fields_ = [("base", C.c_float), ("factor", C.c_float), ("original_len", C.c_int32), ("beta_fast", C.c_float),
+                ("beta_slow", C.c_float)]
+
+    def __init__(self, base, factor=1.0, original_len=0, beta_fast=0.0, beta_slow=0.0):
+        super().__init__(base, factor, original_len, beta_fast, beta_slow)
 
 
 _lib = None
@@ -142,6 +194,13 @@ def lib():
         "spt_ctx_enable_timing": ([vp, C.c_int], C.c_int),
         "spt_ctx_read_timing": ([vp, C.POINTER(C.c_double), C.POINTER(C.c_int64)], C.c_int),
         "spt_upload_range": ([vp, C.c_char_p, u64, u64, T], C.c_int),
+        "spt_kv_cache_bytes": ([C.c_uint32, i32, i32, i32, i64, C.POINTER(u64)], C.c_int),
+        "spt_kv_store_batch": ([vp, C.POINTER(KVCache), C.POINTER(KVBatch), C.POINTER(Rope), vp, i64, vp, i64, vp, i64, vp, i64],
+                               C.c_int),
+        "spt_kv_load_batch": ([vp, C.POINTER(KVCache), C.POINTER(KVBatch), vp, i64, vp, i64], C.c_int),
+        "spt_attention_batch_into": ([vp, C.POINTER(KVCache), C.POINTER(KVBatch), T, C.c_float, i32, vp, i64, vp, i64, vp, vp,
+                                      u64], C.c_int),
+        "spt_attention_work_bytes": ([vp, C.POINTER(KVCache), C.POINTER(KVBatch), i32, i32, C.POINTER(u64)], C.c_int),
         "spt_ctx_memory": ([vp, C.POINTER(u64), C.POINTER(u64)], C.c_int),
     }
     for name, (args, res) in sig.items():
@@ -318,6 +377,32 @@ class Context:
     def rmsnorm_batch_into(self, w: Tensor, x, y, batch: int, eps: float, q8=None):
         _check(lib().spt_rmsnorm_batch_into(self.handle, C.byref(w), _ptr(x), _numel(x), _ptr(y), _numel(y),
                                             batch, eps, _ptr(q8)))
+
+    def kv_store_batch(self, cache: KVCache, batch: KVBatch, k, v, rope: Rope = None, q=None, q_out=None):
+        """Rotate the batch's queries (into q_out) and keys and write keys
+        and values into the cache; rope None: keys as they are, no queries."""
+        nq = _numel(q) if q is not None else 0
+        no = _numel(q_out) if q_out is not None else 0
+        _check(lib().spt_kv_store_batch(self.handle, _ref(cache), _ref(batch), _ref(rope), _ptr(q), nq, _ptr(q_out), no,
+                                        _ptr(k), _numel(k), _ptr(v), _numel(v)))
+
+    def kv_load_batch(self, cache: KVCache, batch: KVBatch, k, v):
+        """The batch's rows of the cache as fp32 keys and values."""
+        _check(lib().spt_kv_load_batch(self.handle, _ref(cache), _ref(batch), _ptr(k), _numel(k), _ptr(v), _numel(v)))
+
+    def attention_work_bytes(self, cache: KVCache, batch: KVBatch, heads: int, window: int = 0) -> int:
+        out = C.c_uint64()
+        _check(lib().spt_attention_work_bytes(self.handle, _ref(cache), _ref(batch), heads, window, C.byref(out)))
+        return out.value
+
+    def attention_batch_into(self, cache: KVCache, batch: KVBatch, q, out, scale: float, window: int = 0, sinks: Tensor = None,
+                             q8=None, work=None):
+        """Attention of the batch's rows over the cache (forwardAttention);
+        q8: GGML Q8_0 blocks of out; work: a uint8 buffer of
+        attention_work_bytes, else the context's arena."""
+        _check(lib().spt_attention_batch_into(self.handle, _ref(cache), _ref(batch), _ref(sinks), scale, window, _ptr(q),
+                                              _numel(q), _ptr(out), _numel(out), _ptr(q8), _ptr(work),
+                                              _numel(work) if work is not None else 0))
 
     def mul_mxfp4_expert(self, w: Tensor, bias, expert: int, x, y, batch: int):
         b = bias if bias is not None else Tensor.absent()
