@@ -1238,9 +1238,13 @@ int kv_check(const spt_kv_cache *c, const spt_kv_batch *b, int *bits, int *nb, s
         return fail(SPT_ERR_INVALID, "key/value batch: %lld positions do not fit %d pages of %d", (long long)b->max_len, b->max_pages, c->page_len);
     if (!b->rows_dev || !b->lens_dev || !b->pages_dev || (((uintptr_t)b->rows_dev | (uintptr_t)b->lens_dev | (uintptr_t)b->pages_dev) & 3))
         return fail(SPT_ERR_INVALID, "key/value batch: nil or unaligned rows, lengths or pages");
+    if (bytes / (uint64_t)c->n_pages > 0x7FFFFFFFull)
+        return fail(SPT_ERR_INVALID, "key/value cache: a page of %llu bytes is too large", (unsigned long long)(bytes / (uint64_t)c->n_pages));
     *bits = kv_type_bits(c->type);
     *nb = c->head_dim / 32;
-    *a = spt::KvArgs{(uint8_t *)c->data, c->n_kv_heads, c->page_len / spt::kKvTile, c->n_pages, b->n_seqs, b->max_new, (int)b->n_rows,
+    const int tiles = c->page_len / spt::kKvTile;
+    *a = spt::KvArgs{(uint8_t *)c->data, c->n_kv_heads, tiles, (uint32_t)((0xFFFFFFFFull + tiles) / tiles),
+                     (int)c->n_pages, b->n_seqs, b->max_new, (int)b->n_rows,
                      (int)b->max_len, b->max_pages, b->rows_dev, b->lens_dev, b->pages_dev};
     return SPT_OK;
 }
@@ -1309,11 +1313,11 @@ int attn_setup(spt_ctx *ctx, const spt_kv_cache *c, const spt_kv_batch *b, int64
     const spt::AttnPlan p = spt::attn_plan(call->nb, c->n_kv_heads, call->a.group, std::max(1, b->n_seqs), b->max_new, (int)b->max_len,
                                            call->a.window, ctx->n_cu > 0 ? ctx->n_cu : 256);
     // a launch holds fewer than 2^32 threads
-    if ((int64_t)p.row_tiles * c->n_kv_heads * p.splits >= (int64_t(1) << 24))
+    if ((int64_t)p.row_tiles * c->n_kv_heads >= (int64_t(1) << 23))
         return fail(SPT_ERR_INVALID, "attention: %d new rows are too many for one call", b->max_new);
+    call->a.unit_rows = p.unit_rows;
     call->a.row_tiles = p.row_tiles;
-    call->a.splits = p.splits;
-    call->a.split_tiles = p.split_tiles;
+    call->a.groups = p.groups;
     call->work_bytes = p.work_bytes;
     return SPT_OK;
 }
@@ -1881,9 +1885,9 @@ int spt_attention_batch_into(spt_ctx *ctx, const spt_kv_cache *cache, const spt_
     call.a.sinks = bias_ptr(sk);
     call.a.sink_type = bias_type(sk);
     call.a.scale = scale * 1.44269504088896341f;
-    call.a.part = (float *)work;
+    call.a.work = work;
     SPT_HIP(timed(ctx, SPT_KERNEL_ATTENTION, [&] { return spt::launch_attn(ctx->stream, call.bits, call.nb, call.a); }));
-    if (call.a.splits > 1) {
+    if (call.a.groups) {
         if ((rc = check_cancel(ctx))) return rc;
         SPT_HIP(timed(ctx, SPT_KERNEL_ATTENTION, [&] { return spt::launch_attn_merge(ctx->stream, call.nb, call.a); }));
     }

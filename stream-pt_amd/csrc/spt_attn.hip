@@ -3,13 +3,15 @@
 // with a head's sink logit in the denominator; grouped heads, causal, with
 // an optional window.
 //
-// Products run on the fp16 MFMA at fp32's accuracy.  A stored value c d (at
-// most 8-bit c, 11-bit d) is exactly the sum of two fp16 numbers: hi =
-// fp16(c d), lo = c d - hi (a multiple of 2^-24, like d; one packed multiply
-// and one packed FMA for two values).  A query row is scaled by a power of
-// two and split the same way (22 bits), and so are the weights p.  Of the four
-// products of halves the three larger are added in fp32; the dropped lo * lo is
-// below 2^-22 of the product.
+// Products run on the fp16 MFMA at fp32's accuracy.  A query row is scaled by
+// a power of two and held as the sum of two fp16 numbers, hi and lo (22 bits);
+// keys enter as their codes, exact in fp16, and a block's scale multiplies its
+// sum.  Weights p are split like queries.  A stored value c d (at most 8-bit c,
+// 11-bit d) is exactly hi + lo, hi = fp16(c d), lo = c d - hi (a multiple of
+// 2^-24, like d; one packed multiply and one packed FMA for two values); of the
+// four products of halves the three larger are added in fp32, the dropped
+// lo * lo being below 2^-22 of the product.  (Scaling the weights by each
+// block's d instead takes as many instructions, and leaves fp16's range.)
 //
 // k_attn_split, rows 16 at a time (a column of the MFMA each; the group's
 // heads of one or more tokens): a wave takes tiles of 32 positions in turn
@@ -20,6 +22,7 @@
 // no exchange between lanes and no rescaling.  The waves' parts meet in LDS;
 // where the rows are few, splits of the positions meet in k_attn_merge.
 #include <algorithm>
+#include <type_traits>
 
 #include "spt_kernels.h"
 #include "spt_kv.h"
@@ -34,7 +37,17 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kAttnRows = 16;           // rows of a row tile
-constexpr int kWaves = 4;
+#ifndef WAVES
+#define WAVES 8
+#endif
+constexpr int kWaves = WAVES;           // of a workgroup
+constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup sums up
+#ifndef FEW
+#define FEW 32
+#define UNITCOST 8
+#endif
+constexpr int kFewRows = FEW;       // up to so many rows of a key/value head: kAttnRows at a time
+constexpr int kDirectTiles = 16;    // a unit of up to so many position tiles is one workgroup's
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
 constexpr float kLift = 5.0f;       // weights are held times 2^kLift (at most 2^13)
@@ -49,25 +62,80 @@ __device__ inline half2v pk(uint32_t w) { return __builtin_bit_cast(half2v, w); 
 // Codes of eight positions or dims as fp16 pairs.  Q4_0: w's low nibbles (or
 // high) of bytes 0 and 2, then 1 and 3, into the low mantissa bits of 1024
 // (or 16 places higher, 64 + n after the multiply by 1/16).
-__device__ inline half2v q4_low(uint32_t w) { return pk((w & 0x000F000Fu) | 0x64006400u) + (half2v)(_Float16)-1032.0f; }
-__device__ inline half2v q4_high(uint32_t w) {
-    return __builtin_elementwise_fma(pk((w & 0x00F000F0u) | 0x64006400u), (half2v)(_Float16)0.0625f, (half2v)(_Float16)-72.0f);
+// Constants that the compiler does not see through: with them it makes one
+// v_and_or_b32 of the mask and the or, and one mixed-precision FMA of a
+// conversion and a product or sum, where it would fold known ones apart.
+struct Opaque {
+    uint32_t low = 0x000F000Fu, high = 0x00F000F0u, k1024 = 0x64006400u;
+    float zero = 0.0f, minus = -1.0f;
+    __device__ inline Opaque() {
+        asm("" : "+s"(low));
+        asm("" : "+s"(high));
+        asm("" : "+v"(k1024));
+        asm("" : "+v"(zero));
+        asm("" : "+v"(minus));
+    }
+};
+
+__device__ inline half2v q4_low(const Opaque &o, uint32_t w) { return pk((w & o.low) | o.k1024) + (half2v)(_Float16)-1032.0f; }
+__device__ inline half2v q4_high(const Opaque &o, uint32_t w) {
+    return __builtin_elementwise_fma(pk((w & o.high) | o.k1024), (half2v)(_Float16)0.0625f, (half2v)(_Float16)-72.0f);
 }
 __device__ inline half2v q8_pair(uint32_t w, int upper) {
     return pk(__builtin_amdgcn_perm(0x64646464u, w, upper ? 0x04030402u : 0x04010400u)) + (half2v)(_Float16)-1152.0f;
 }
 
-// The codes' values, split.
-__device__ inline void split_values(const half2v (&c)[4], const half2v (&d)[4], Half8 &hi, Half8 &lo) {
+// The key operand of a Q4_0 word, and the value operand of two (dims 16 h on).
+__device__ inline void q4_key(const Opaque &o, uint32_t w, Half8 &c) {
+    const uint32_t x = w >> 8;
+    c.h[0] = q4_low(o, w);
+    c.h[1] = q4_high(o, w);
+    c.h[2] = q4_low(o, x);
+    c.h[3] = q4_high(o, x);
+}
+__device__ inline void q4_value(const Opaque &o, uint32_t w0, uint32_t w1, int h, Half8 &c) {
+    const uint32_t x0 = w0 >> 8, x1 = w1 >> 8;
+    c.h[0] = h ? q4_high(o, w0) : q4_low(o, w0);
+    c.h[1] = h ? q4_high(o, x0) : q4_low(o, x0);
+    c.h[2] = h ? q4_high(o, w1) : q4_low(o, w1);
+    c.h[3] = h ? q4_high(o, x1) : q4_low(o, x1);
+}
+// Either operand of two Q8_0 words.
+__device__ inline void q8_codes(uint32_t w0, uint32_t w1, Half8 &c) {
+    c.h[0] = q8_pair(w0, 0);
+    c.h[1] = q8_pair(w0, 1);
+    c.h[2] = q8_pair(w1, 0);
+    c.h[3] = q8_pair(w1, 1);
+}
+
+// The codes' values, split; d: the scales of eight positions.
+__device__ inline void split_values(const Half8 &c, const u32x4 &d, Half8 &hi, Half8 &lo) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        hi.h[i] = c[i] * d[i];
-        lo.h[i] = __builtin_elementwise_fma(c[i], d[i], -hi.h[i]);
+        hi.h[i] = c.h[i] * pk(d[i]);
+        lo.h[i] = __builtin_elementwise_fma(c.h[i], pk(d[i]), -hi.h[i]);
     }
+}
+
+// The scales of eight positions, 0 from the one `left` on.
+__device__ inline void clear_scales(u32x4 &d, int left) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = left <= 2 * i ? 0u : left == 2 * i + 1 ? d[i] & 0xFFFFu : d[i];
+}
+__device__ inline u32x4 load16(rsrc_t tile, int lane_at, int at) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(tile, lane_at, at, 0));
 }
 
 __device__ inline f32x4 mfma(const Half8 &a, const Half8 &b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
+}
+
+// Two fp32 numbers as hi + lo: hi rounded toward zero, lo what that leaves
+// (x - hi, rounded once).
+__device__ inline void split_pair(const Opaque &o, float x, float y, half2v &hi, half2v &lo) {
+    hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x, y));
+    lo[0] = (_Float16)__builtin_fmaf((float)hi[0], o.minus, x);
+    lo[1] = (_Float16)__builtin_fmaf((float)hi[1], o.minus, y);
 }
 
 // A lane's raw bytes of a tile.
@@ -75,101 +143,143 @@ template <int BITS, int NB>
 struct RawTile {
     static constexpr int kUnits = BITS == 4 ? NB / 2 : NB;
     u32x4 k[kUnits], v[kUnits];
-    uint32_t ks[NB];      // key scales [t][b], two fp16 a word
+    u32x4 ks[NB];         // key scales of positions 8 g + i + 4 t: [i][t][b]
     u32x4 vs[NB];         // value scales of 8 positions
 
-    __device__ inline void load_keys(const uint8_t *tile, int lane) {
+    // From a tile's descriptor: of no bytes where there is no tile, and then all is 0.
+    __device__ inline void load(rsrc_t tile, int lane) {
         using T = KvTile<BITS, NB>;
+        const int l16 = lane * 16, g16 = (lane >> 4) * 16;
 #pragma unroll
-        for (int u = 0; u < kUnits; u++) k[u] = *reinterpret_cast<const u32x4 *>(tile + (u * 64 + lane) * 16);
+        for (int u = 0; u < kUnits; u++) k[u] = load16(tile, l16, u * 1024);
 #pragma unroll
-        for (int i = 0; i < NB; i += 2) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(tile + T::kScales + (lane & 15) * 4 * NB + i * 4);
-            ks[i] = x.x;
-            ks[i + 1] = x.y;
-        }
+        for (int i = 0; i < NB; i++) ks[i] = load16(tile, g16 * NB, T::kScales + i * 16);
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) v[u] = load16(tile, l16, T::kValues + u * 1024);
+#pragma unroll
+        for (int b = 0; b < NB; b++) vs[b] = load16(tile, g16, T::kValues + T::kScales + b * 64);
     }
-    __device__ inline void load_values(const uint8_t *tile, int lane) {
-        using T = KvTile<BITS, NB>;
-#pragma unroll
-        for (int u = 0; u < kUnits; u++) v[u] = *reinterpret_cast<const u32x4 *>(tile + T::kValues + (u * 64 + lane) * 16);
-#pragma unroll
-        for (int b = 0; b < NB; b++) vs[b] = *reinterpret_cast<const u32x4 *>(tile + T::kValues + T::kScales + b * 64 + (lane >> 4) * 16);
-    }
-    // Key operand of tile half t, block b.
-    __device__ inline void keys(int t, int b, Half8 &hi, Half8 &lo) const {
-        half2v c[4], d[4];
+    // Key operand of tile half t, block b: the codes.
+    __device__ inline void keys(const Opaque &o, int t, int b, Half8 &c) const {
         if (BITS == 4) {
-            const uint32_t w = k[b >> 1][t * 2 + (b & 1)], x = w >> 8;
-            c[0] = q4_low(w);
-            c[1] = q4_high(w);
-            c[2] = q4_low(x);
-            c[3] = q4_high(x);
+            q4_key(o, k[b >> 1][t * 2 + (b & 1)], c);
         } else {
             const u32x4 &u = k[(b >> 1) * 2 + t];
-            const uint32_t w0 = u[(b & 1) * 2], w1 = u[(b & 1) * 2 + 1];
-            c[0] = q8_pair(w0, 0);
-            c[1] = q8_pair(w0, 1);
-            c[2] = q8_pair(w1, 0);
-            c[3] = q8_pair(w1, 1);
+            q8_codes(u[(b & 1) * 2], u[(b & 1) * 2 + 1], c);
         }
-        const half2v s = pk(ks[(t * NB + b) >> 1]);
-        const half2v dd = (b & 1) ? half2v{s[1], s[1]} : half2v{s[0], s[0]};
-#pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = dd;
-        split_values(c, d, hi, lo);
+    }
+    // s times the scale of position 8 g + 4 t + i, block b, plus c.
+    __device__ inline float scaled(float s, int t, int i, int b, float c) const {
+        const int h = (i * 2 + t) * NB + b;
+        return __builtin_fmaf(s, (float)pk(ks[h >> 3][h >> 1 & 3])[h & 1], c);
     }
     // Value operand of block b, dims 16 h .. 16 h + 15.
-    __device__ inline void values(int b, int h, Half8 &hi, Half8 &lo) const {
-        half2v c[4], d[4];
-        if (BITS == 4) {
-            const uint32_t w0 = v[b >> 1][(b & 1) * 2], w1 = v[b >> 1][(b & 1) * 2 + 1];
-            c[0] = h ? q4_high(w0) : q4_low(w0);
-            c[1] = h ? q4_high(w0 >> 8) : q4_low(w0 >> 8);
-            c[2] = h ? q4_high(w1) : q4_low(w1);
-            c[3] = h ? q4_high(w1 >> 8) : q4_low(w1 >> 8);
-        } else {
-            const uint32_t w0 = v[b][h * 2], w1 = v[b][h * 2 + 1];
-            c[0] = q8_pair(w0, 0);
-            c[1] = q8_pair(w0, 1);
-            c[2] = q8_pair(w1, 0);
-            c[3] = q8_pair(w1, 1);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = pk(vs[b][i]);
-        split_values(c, d, hi, lo);
+    __device__ inline void values(const Opaque &o, int b, int h, Half8 &hi, Half8 &lo) const {
+        Half8 c;
+        if (BITS == 4)
+            q4_value(o, v[b >> 1][(b & 1) * 2], v[b >> 1][(b & 1) * 2 + 1], h, c);
+        else
+            q8_codes(v[b][h * 2], v[b][h * 2 + 1], c);
+        split_values(c, vs[b], hi, lo);
     }
     // Positions from `left` on (of the lane's eight, at 8 g) are beyond the
     // sequence: whatever is there counts as zero.
     __device__ inline void clear_values(int left) {
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) vs[b][i] = left <= 2 * i ? 0u : left == 2 * i + 1 ? vs[b][i] & 0xFFFFu : vs[b][i];
+        for (int b = 0; b < NB; b++) clear_scales(vs[b], left);
     }
 };
 
-// What a row tile's rows see: positions [0, ..] of the first and the last row,
-// and the tiles that hold any of them.
-struct RowSpan {
-    int i_first, i_last;  // tokens
-    int t_lo, t_hi;       // tiles
+#ifndef AHEAD
+#define AHEAD (NB == 4)
+#endif
+// Whether a tile is loaded while another is taken, and the waves a SIMD that
+// registers have to leave room for.
+template <int BITS, int NB>
+constexpr bool kAhead = AHEAD;
+template <int NB>
+#ifndef MINW
+#define MINW 4
+#endif
+constexpr int kMinWaves = NB == 2 ? MINW : 2;
+
+// A unit of work: a row tile (kAttnRows or kManyRows rows) of a sequence and a
+// key/value head.  Its rows
+// are tokens [i_first, i_last]; the tiles [t_lo, t_hi) hold what they see.
+struct Unit {
+    KvSeq sq;
+    int rows, i_first, i_last, t_lo, t_hi;
+    __device__ inline int tiles() const { return max(1, t_hi - t_lo); }  // one that sees nothing is written too
 };
 
-__device__ inline RowSpan row_span(const AttnArgs &a, const KvSeq &sq, int rt) {
-    RowSpan r;
-    const int rows = sq.n * a.group;
-    r.i_first = rt * kAttnRows / a.group;
-    r.i_last = (min(rows, rt * kAttnRows + kAttnRows) - 1) / a.group;
-    const int last = sq.first + r.i_last;
-    const int lo = a.window ? max(0, sq.first + r.i_first - a.window + 1) : 0;
-    r.t_lo = lo / kKvTile;
-    r.t_hi = last < 0 ? r.t_lo : last / kKvTile + 1;
-    return r;
+// Row tile rt of a sequence; rows is 0 where it has none.
+template <int ROWS>
+__device__ inline Unit unit_of(const AttnArgs &a, const KvSeq &sq, int rt) {
+    Unit u;
+    u.sq = sq;
+    u.rows = min(ROWS, u.sq.n * a.group - rt * ROWS);
+    if (u.rows <= 0) {
+        u.rows = u.i_first = u.i_last = u.t_lo = u.t_hi = 0;
+        return u;
+    }
+    u.i_first = rt * ROWS / a.group;
+    u.i_last = (rt * ROWS + u.rows - 1) / a.group;
+    const int last = u.sq.first + u.i_last;
+    const int lo = a.window ? max(0, u.sq.first + u.i_first - a.window + 1) : 0;
+    u.t_lo = lo / kKvTile;
+    u.t_hi = last < 0 ? u.t_lo : last / kKvTile + 1;
+    if (!u.sq.ok) u.t_lo = u.t_hi = 0;
+    return u;
 }
 
-__device__ inline int active_splits(const AttnArgs &a, const RowSpan &r) {
-    return max(1, (r.t_hi - r.t_lo + a.split_tiles - 1) / a.split_tiles);
+// The places of tiles t, t + step, .. of a sequence and head, in scalar
+// registers; a page past the table is none.
+struct TileWalk {
+    struct Place {
+        int page, tile;
+    };
+    KvConst table;
+    uint32_t page_bytes, head_bytes, n_pages;
+    int tile_bytes, page_tiles, max_pages, at, tile, at_step, tile_step;
+
+    __device__ inline TileWalk(const KvArgs &a, int seq, int head, int t, int step, int bytes) {
+        table = kv_const(a.pages) + (int64_t)seq * a.max_pages;
+        page_tiles = a.page_tiles;
+        tile_bytes = bytes;
+        head_bytes = (uint32_t)head * page_tiles * bytes;
+        page_bytes = (uint32_t)a.kv_heads * page_tiles * bytes;
+        n_pages = (uint32_t)a.n_pages;
+        max_pages = a.max_pages;
+        at = kv_page_of(a, t, &tile);
+        at_step = kv_page_of(a, step, &tile_step);
+    }
+    __device__ inline Place next() {
+        const Place p{at < max_pages ? table[at] : -1, tile};
+        at += at_step;
+        tile += tile_step;
+        if (tile >= page_tiles) tile -= page_tiles, at++;
+        return p;
+    }
+    __device__ inline bool ok(const Place &p) const { return (uint32_t)p.page < n_pages; }
+    __device__ inline uint64_t offset(const Place &p) const {
+        return (uint64_t)(uint32_t)p.page * page_bytes + (head_bytes + (uint32_t)(p.tile * tile_bytes));
+    }
+};
+
+// The workspace: each unit's first and last part, each part's (maximum, sum)
+// of its rows, and its rows' partial outputs.
+struct AttnWork {
+    int2 *units;
+    float2 *tops;  // [part][unit_rows]
+    float *outs;   // [part][unit_rows][dim]
+};
+__device__ inline AttnWork attn_work(const AttnArgs &a) {
+    const int64_t units = (int64_t)a.kv.n_seqs * a.row_tiles * a.kv.kv_heads;
+    AttnWork w;
+    w.units = reinterpret_cast<int2 *>(a.work);
+    w.tops = reinterpret_cast<float2 *>(w.units + units);
+    w.outs = reinterpret_cast<float *>(w.tops + (a.groups + units) * a.unit_rows);
+    return w;
 }
 
 // Sink, division and stores of a row's block of 32 (an element a lane of a
@@ -192,90 +302,108 @@ __device__ inline void store_row(const AttnArgs &a, int head, int64_t row, int b
     }
 }
 
-template <int BITS, int NB>
-__global__ __launch_bounds__(64 * kWaves) void k_attn_split(AttnArgs a) {
-    using T = KvTile<BITS, NB>;
-    constexpr int kDim = 32 * NB;
-    __shared__ float so[kWaves][kAttnRows][kDim + 4];
-    __shared__ float sm[kWaves][kAttnRows], sl[kWaves][kAttnRows];
-    const int seq = blockIdx.y;
-    const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
-    const int kvh = unit % a.kv.kv_heads, rt = unit / a.kv.kv_heads;
-    const KvSeq sq = kv_seq(a.kv, seq);
-    const int rows = sq.n * a.group;
-    if (rt * kAttnRows >= rows) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
-    RowSpan sp = row_span(a, sq, rt);
-    if (!sq.ok) sp.t_lo = sp.t_hi = 0;
-    if (split >= active_splits(a, sp)) return;
-
-    // the row of this lane's column
-    const int flat = rt * kAttnRows + col;
-    const bool row_ok = flat < rows;
-    const int tok = row_ok ? flat / a.group : sp.i_last, hd = kvh * a.group + (row_ok ? flat % a.group : 0);
-    const int pos = sq.first + tok;                    // last position that it sees
-    const int from = a.window ? pos - a.window : -1;   // it sees those after this one
-
-    Half8 qh[NB], ql[NB];
+// A row of queries as the B operand, times the softmax scale, hi and lo; the
+// products are scores (times log2 e) divided by mul.
+template <int NB>
+struct Query {
+    Half8 hi[NB], lo[NB];
     float mul;
-    {
+    __device__ inline void load(const AttnArgs &a, int64_t row, int head, int g) {
         float x[NB][8], top = 0.0f;
-        const float *src = a.q + ((int64_t)(sq.r0 + tok) * a.heads + hd) * kDim + 8 * g;
+        const float *src = a.q + (row * a.heads + head) * 32 * NB + 8 * g;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             const float4 u = *reinterpret_cast<const float4 *>(src + 32 * b), w = *reinterpret_cast<const float4 *>(src + 32 * b + 4);
             x[b][0] = u.x, x[b][1] = u.y, x[b][2] = u.z, x[b][3] = u.w;
             x[b][4] = w.x, x[b][5] = w.y, x[b][6] = w.z, x[b][7] = w.w;
 #pragma unroll
+            for (int i = 0; i < 8; i++) x[b][i] *= a.scale;
+#pragma unroll
             for (int i = 0; i < 8; i++) top = fmaxf(top, __builtin_fabsf(x[b][i]));
         }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const int e = __builtin_amdgcn_frexp_expf(top);
-        mul = __builtin_ldexpf(a.scale, e - 13);
+        // mul is a power of two, so that scores times it are exact: the largest
+        // minus the maximum is 0 however large they are.  (Not so small that it
+        // is 0: it multiplies the -inf of hidden positions.)
+        const int e = max(-100, __builtin_amdgcn_frexp_expf(top));
+        mul = __builtin_ldexpf(1.0f, e - 13);
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float y = __builtin_ldexpf(x[b][i], 13 - e);
-                qh[b].v[i] = (_Float16)y;
-                ql[b].v[i] = (_Float16)(y - (float)qh[b].v[i]);
+                hi[b].v[i] = (_Float16)y;
+                lo[b].v[i] = (_Float16)(y - (float)hi[b].v[i]);
             }
     }
+};
 
+template <int NB>
+struct AttnLds {
+    float o[kWaves][kAttnRows][32 * NB + 4];
+    float m[kWaves][kAttnRows], l[kWaves][kAttnRows];
+};
+
+// Tiles [t_begin, t_end) of a unit by the workgroup; the result is the unit's
+// own (part < 0), or that part of it.
+template <int BITS, int NB>
+__device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, const Unit &un, int seq, int rt, int kvh, int t_begin, int t_end,
+                                                             int64_t part, AttnLds<NB> &lds) {
+    using T = KvTile<BITS, NB>;
+    constexpr int kDim = 32 * NB;
+    const KvSeq &sq = un.sq;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int t = t_begin + wave;
+    TileWalk walk(a.kv, seq, kvh, t, kWaves, T::kBytes);
+    // Loads are issued on every path: the compiler waits for all of them where
+    // paths join.
+    auto load = [&](RawTile<BITS, NB> &raw, const TileWalk::Place &p) __attribute__((always_inline)) {
+        raw.load(__builtin_amdgcn_make_buffer_rsrc(a.kv.data + walk.offset(p), (short)0, walk.ok(p) ? T::kBytes : 0, kRsrcWord3), lane);
+    };
+    RawTile<BITS, NB> even;
+    TileWalk::Place p0 = walk.next(), p1 = walk.next();
+    load(even, p0);
+
+    // the row of this lane's column
+    const int flat = rt * kAttnRows + col;
+    const bool row_ok = col < un.rows;
+    const int tok = row_ok ? flat / a.group : un.i_last, hd = kvh * a.group + (row_ok ? flat % a.group : 0);
+    const int pos = sq.first + tok;                   // last position that it sees
+    const int from = a.window ? pos - a.window : -1;  // it sees those after this one
+
+    Query<NB> q;
+    q.load(a, sq.r0 + tok, hd, g);
+
+    const Opaque oc;
     f32x4 o[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = kNoMax, l = sq.ok ? 0.0f : __builtin_nanf("");
-    const int t_end = min(sp.t_hi, sp.t_lo + (split + 1) * a.split_tiles);
-    for (int t = sp.t_lo + split * a.split_tiles + wave; t < t_end; t += kWaves) {
+    // A tile's part, from its bytes in registers.
+    auto take = [&](RawTile<BITS, NB> &raw, const TileWalk::Place &at) __attribute__((always_inline)) {
         const int p0 = t * kKvTile;
-        const uint8_t *tile = kv_tile(a.kv, seq, kvh, t, T::kBytes);
-        if (!tile) {
+        if (!walk.ok(at)) {
             if (p0 <= pos && p0 + kKvTile - 1 > from) l = __builtin_nanf("");
-            continue;
+            return;
         }
-        RawTile<BITS, NB> raw;
-        raw.load_keys(tile, lane);
-        raw.load_values(tile, lane);
-        f32x4 s[2];
+        float x[8] = {}, top = -__builtin_inff();
+        const bool whole = p0 + kKvTile - 1 <= sq.first + un.i_first && (!a.window || p0 > sq.first + un.i_last - a.window);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                Half8 kh, kl;
-                raw.keys(h, b, kh, kl);
-                s[h] = mfma(kh, qh[b], s[h]);
-                s[h] = mfma(kh, ql[b], s[h]);
-                s[h] = mfma(kl, qh[b], s[h]);
+                Half8 c;
+                raw.keys(oc, h, b, c);
+                f32x4 s = mfma(c, q.hi[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                s = mfma(c, q.lo[b], s);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[4 * h + i] = raw.scaled(s[i], h, i, b, b ? x[4 * h + i] : oc.zero);
             }
         }
-        float x[8], top = -__builtin_inff();
-        const bool whole = p0 + kKvTile - 1 <= sq.first + sp.i_first && (!a.window || p0 > sq.first + sp.i_last - a.window);
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * mul;
         if (!whole) {
+            asm volatile("");  // a branch: the whole tiles, nearly all, do without
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int p = p0 + 8 * g + j;
@@ -285,6 +413,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_split(AttnArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) top = fmaxf(top, x[j]);
+        top *= q.mul;
         if (__any(top > m + kSlack)) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
@@ -295,122 +424,542 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_split(AttnArgs a) {
             for (int b = 0; b < NB; b++) o[b][0] *= f, o[b][1] *= f;
         }
         Half8 ph, pl;
+        const float back = kLift - m;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float w = __builtin_amdgcn_exp2f(x[j] - (m - kLift));
-            l += w;
-            ph.v[j] = (_Float16)w;
-            pl.v[j] = (_Float16)(w - (float)ph.v[j]);
+        for (int j = 0; j < 8; j += 2) {
+            const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], q.mul, back)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j + 1], q.mul, back));
+            l += w0;
+            l += w1;
+            split_pair(oc, w0, w1, ph.h[j >> 1], pl.h[j >> 1]);
         }
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 Half8 vh, vl;
-                raw.values(b, h, vh, vl);
+                raw.values(oc, b, h, vh, vl);
                 o[b][h] = mfma(vh, ph, o[b][h]);
                 o[b][h] = mfma(vh, pl, o[b][h]);
                 o[b][h] = mfma(vl, ph, o[b][h]);
             }
+    };
+    if (kAhead<BITS, NB>) {
+        // two tiles in registers, one being loaded while the other is taken
+        RawTile<BITS, NB> odd;
+        while (t < t_end) {
+            load(odd, p1);
+            const TileWalk::Place p2 = walk.next();
+            take(even, p0);
+            t += kWaves;
+            if (t >= t_end) break;
+            load(even, p2);
+            const TileWalk::Place p3 = walk.next();
+            take(odd, p1);
+            t += kWaves;
+            p0 = p2;
+            p1 = p3;
+        }
+    } else {
+        for (; t < t_end; t += kWaves) {
+            take(even, p0);
+            p0 = p1;
+            p1 = walk.next();
+            load(even, p0);
+        }
     }
 
     // the waves' parts, on the largest maximum
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) sm[wave][col] = m, sl[wave][col] = l;
+    if (g == 0) lds.m[wave][col] = m, lds.l[wave][col] = l;
     __syncthreads();
-    float top = sm[0][col];
+    float top = lds.m[0][col];
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) top = fmaxf(top, sm[w][col]);
+    for (int w = 1; w < kWaves; w++) top = fmaxf(top, lds.m[w][col]);
     const float f = __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&so[wave][col][32 * b + 16 * h + 4 * g]) = o[b][h] * f;
+        for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&lds.o[wave][col][32 * b + 16 * h + 4 * g]) = o[b][h] * f;
     __syncthreads();
     // a half-wave takes a block of a row
     for (int u = wave * 2 + (lane >> 5); u < kAttnRows * NB; u += 2 * kWaves) {
         const int r = u / NB, b = u % NB, d = 32 * b + (lane & 31);
-        float mx = sm[0][r], sum = 0.0f, den = 0.0f;
+        float mx = lds.m[0][r], sum = 0.0f, den = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, sm[w][r]);
+        for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, lds.m[w][r]);
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-            den += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - mx);
-            sum += so[w][r][d];
+            den += lds.l[w][r] * __builtin_amdgcn_exp2f(lds.m[w][r] - mx);
+            sum += lds.o[w][r][d];
         }
+        mx -= kLift;  // weights are 2^kLift too large, the sink is not
         const int fr = rt * kAttnRows + r;
-        const bool ok = fr < rows;
-        if (a.splits == 1) {
-            // the weights are 2^kLift too large on both sides; the sink is not
-            store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, b, NB, sum, den, mx - kLift, lane, ok);
+        const bool ok = r < un.rows;
+        if (part < 0) {
+            store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, b, NB, sum, den, mx, lane, ok);
         } else if (ok) {
-            float *part = a.part + (((int64_t)seq * a.row_tiles * a.kv.kv_heads + unit) * a.splits + split) * kAttnRows * (kDim + 2);
-            part[r * (kDim + 2) + 2 + d] = sum;
-            if (d == 0) part[r * (kDim + 2)] = mx - kLift, part[r * (kDim + 2) + 1] = den;
+            const AttnWork w = attn_work(a);
+            w.outs[(part * kAttnRows + r) * kDim + d] = sum;
+            if (d == 0) w.tops[part * kAttnRows + r] = make_float2(mx, den);
         }
     }
 }
 
-// The splits of a row tile: a wave takes rows in turn, a half-wave a block.
+// A workgroup a unit.
+template <int BITS, int NB>
+__global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_units(AttnArgs a) {
+    __shared__ AttnLds<NB> lds;
+    const int kvh = blockIdx.x % a.kv.kv_heads, rt = blockIdx.x / a.kv.kv_heads, seq = blockIdx.y;
+    const Unit u = unit_of<kAttnRows>(a, kv_seq(a.kv, seq), rt);
+    if (u.rows) attend<BITS, NB>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
+}
+
+// Rows many at a time: a workgroup's 8 waves have 32 rows each (two columns of
+// the MFMA), and share the tiles' operands, made once a workgroup in LDS: key
+// codes, and values as hi and lo.  While one tile is taken from one buffer, the
+// next is made in the other and the bytes of the one after it are on their
+// way.  Each wave makes an eighth of a tile: a unit is a key or value operand of
+// one MFMA, 1 KB or twice 1 KB.
+constexpr int kManyWaves = 8, kManyRows = 32 * kManyWaves;
+
 template <int NB>
-__global__ __launch_bounds__(256) void k_attn_merge(AttnArgs a) {
-    constexpr int kDim = 32 * NB;
-    const int seq = blockIdx.y, unit = blockIdx.x, kvh = unit % a.kv.kv_heads, rt = unit / a.kv.kv_heads;
-    const KvSeq sq = kv_seq(a.kv, seq);
-    const int rows = sq.n * a.group;
-    if (rt * kAttnRows >= rows) return;
-    RowSpan sp = row_span(a, sq, rt);
-    if (!sq.ok) sp.t_lo = sp.t_hi = 0;
-    const int n = active_splits(a, sp), lane = threadIdx.x & 63;
-    const float *base = a.part + ((int64_t)seq * a.row_tiles * a.kv.kv_heads + unit) * a.splits * kAttnRows * (kDim + 2);
-    for (int u = threadIdx.x >> 5; u < kAttnRows * NB; u += 8) {
-        const int r = u / NB, b = u % NB, fr = rt * kAttnRows + r;
-        const bool ok = fr < rows;
-        float m = kNoMax, l = 0.0f, o = 0.0f;
-        for (int i = 0; ok && i < n; i++) {
-            const float *p = base + ((int64_t)i * kAttnRows + r) * (kDim + 2);
-            const float pm = p[0], top = fmaxf(m, pm), f = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(pm - top);
-            l = l * f + p[1] * w;
-            o = o * f + p[2 + 32 * b + (lane & 31)] * w;
-            m = top;
-        }
-        store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, b, NB, o, l, m, lane, ok);
+union ManyLds {
+    struct Buffer {
+        Half8 k[2 * NB][64];     // [t][b][lane]
+        Half8 v[2 * NB][2][64];  // [b][h][hi, lo][lane]
+        u32x4 ks[4 * NB];        // scales as they are stored
+    } buf[2];
+    struct {
+        float o[kManyWaves][kAttnRows][32 * NB + 4];
+        float m[kManyWaves][kAttnRows], l[kManyWaves][kAttnRows];
+    } end;
+};
+
+// A wave's part of a tile: NB / 2 units of keys (waves 0 to 3) or values.
+template <int BITS, int NB>
+struct ManyPart {
+    static constexpr int kUnits = NB / 2;
+    uint2 c[kUnits];
+    u32x4 d[kUnits];  // values: scales of eight positions; keys: all scales, by the first lanes
+    bool ok;
+
+    static __device__ inline uint2 load8(rsrc_t tile, int lane_at, int at) {
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(tile, lane_at, at, 0));
     }
+    __device__ inline void load(rsrc_t tile, bool page_ok, int wave, int lane) {
+        using T = KvTile<BITS, NB>;
+        ok = page_ok;
+#pragma unroll
+        for (int j = 0; j < kUnits; j++) {
+            const int u = (wave & 3) * kUnits + j;
+            if (wave < 4) {
+                const int t = u / NB, b = u % NB;
+                if (BITS == 4)
+                    c[j].x = __builtin_amdgcn_raw_buffer_load_b32(tile, lane * 16, (b >> 1) * 1024 + t * 8 + (b & 1) * 4, 0);
+                else
+                    c[j] = load8(tile, lane * 16, ((b >> 1) * 2 + t) * 1024 + (b & 1) * 8);
+                if (j == 0) d[j] = load16(tile, (lane & (4 * NB - 1)) * 16, T::kScales);
+            } else {
+                const int b = u >> 1, h = u & 1;
+                c[j] = BITS == 4 ? load8(tile, lane * 16, T::kValues + (b >> 1) * 1024 + (b & 1) * 8)
+                                 : load8(tile, lane * 16, T::kValues + b * 1024 + h * 8);
+                d[j] = load16(tile, (lane >> 4) * 16, T::kValues + T::kScales + b * 64);
+            }
+        }
+    }
+    // left: positions of the tile before the sequence's end.
+    __device__ inline void make(const Opaque &o, typename ManyLds<NB>::Buffer &buf, int left, int wave, int lane) {
+#pragma unroll
+        for (int j = 0; j < kUnits; j++) {
+            const int u = (wave & 3) * kUnits + j;
+            if (wave < 4) {
+                Half8 k;
+                if (BITS == 4)
+                    q4_key(o, c[j].x, k);
+                else
+                    q8_codes(c[j].x, c[j].y, k);
+                buf.k[u][lane] = k;
+                // no page: the scores are NaN
+                if (u == 0 && lane < 4 * NB) buf.ks[lane] = ok ? d[j] : u32x4{0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u};
+            } else {
+                Half8 v, hi, lo;
+                if (BITS == 4) {
+                    q4_value(o, c[j].x, c[j].y, 0, v);
+                    if (u & 1) q4_value(o, c[j].x, c[j].y, 1, v);
+                } else {
+                    q8_codes(c[j].x, c[j].y, v);
+                }
+                if (left < kKvTile) clear_scales(d[j], left - 8 * (lane >> 4));
+                split_values(v, d[j], hi, lo);
+                buf.v[u][0][lane] = hi;
+                buf.v[u][1][lane] = lo;
+            }
+        }
+    }
+};
+
+template <int BITS, int NB>
+__device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs &a, const Unit &un, int seq, int rt, int kvh, int t_begin,
+                                                                  int t_end, int64_t part, ManyLds<NB> &lds) {
+    using T = KvTile<BITS, NB>;
+    constexpr int kDim = 32 * NB;
+    const KvSeq &sq = un.sq;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    TileWalk walk(a.kv, seq, kvh, t_begin, 1, T::kBytes);
+    ManyPart<BITS, NB> raw;
+    auto load = [&]() __attribute__((always_inline)) {
+        const TileWalk::Place p = walk.next();
+        const bool ok = walk.ok(p);
+        raw.load(__builtin_amdgcn_make_buffer_rsrc(a.kv.data + walk.offset(p), (short)0, ok ? T::kBytes : 0, kRsrcWord3), ok, wave, lane);
+    };
+    load();
+
+    // this wave's rows: two columns' rows a lane
+    const int row0 = rt * kManyRows + wave * 32, rows = un.rows - wave * 32;
+    const int i0 = row0 / a.group, i1 = (row0 + min(rows, 32) - 1) / a.group;  // its tokens
+    const int pos0 = sq.first + i0, pos1 = sq.first + i1;
+    int pos[2], from[2];
+    Query<NB> q[2];
+    f32x4 o[2][NB][2];
+    float m[2] = {kNoMax, kNoMax}, l[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const int r = 16 * c + col;
+        const bool ok = r < rows;
+        const int tok = ok ? (row0 + r) / a.group : un.i_last, hd = kvh * a.group + (ok ? (row0 + r) % a.group : 0);
+        pos[c] = sq.first + tok;
+        from[c] = a.window ? pos[c] - a.window : -1;
+        q[c].load(a, sq.r0 + tok, hd, g);
+        l[c] = sq.ok ? 0.0f : __builtin_nanf("");
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[c][b][0] = o[c][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const Opaque oc;
+
+    auto take = [&](const typename ManyLds<NB>::Buffer &buf, int t) __attribute__((always_inline)) {
+        const int p0 = t * kKvTile;
+        // nothing here is for this wave's rows
+        if (rows <= 0 || p0 > pos1 || (a.window && p0 + kKvTile - 1 <= pos0 - a.window)) return;
+        const bool whole = p0 + kKvTile - 1 <= pos0 && (!a.window || p0 > pos1 - a.window);
+        u32x4 ks[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i++) ks[i] = buf.ks[g * NB + i];
+        float x[2][8];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const Half8 k = buf.k[h * NB + b][lane];
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    f32x4 s = mfma(k, q[c].hi[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                    s = mfma(k, q[c].lo[b], s);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int n = (i * 2 + h) * NB + b;
+                        x[c][4 * h + i] = __builtin_fmaf(s[i], (float)pk(ks[n >> 3][n >> 1 & 3])[n & 1], b ? x[c][4 * h + i] : oc.zero);
+                    }
+                }
+            }
+        if (!whole) {
+            asm volatile("");
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int p = p0 + 8 * g + j;
+                    x[c][j] = p <= pos[c] && p > from[c] ? x[c][j] : -__builtin_inff();
+                }
+        }
+        float top[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            top[c] = x[c][0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) top[c] = fmaxf(top[c], x[c][j]);
+            top[c] *= q[c].mul;
+        }
+        if (__any(top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                top[c] = fmaxf(top[c], __shfl_xor(top[c], 16));
+                top[c] = fmaxf(top[c], __shfl_xor(top[c], 32));
+                const float nm = fmaxf(m[c], top[c]), f = __builtin_amdgcn_exp2f(m[c] - nm);
+                m[c] = nm;
+                l[c] *= f;
+#pragma unroll
+                for (int b = 0; b < NB; b++) o[c][b][0] *= f, o[c][b][1] *= f;
+            }
+        }
+        Half8 ph[2], pl[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const float back = kLift - m[c];
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][j], q[c].mul, back));
+                const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][j + 1], q[c].mul, back));
+                l[c] += w0;
+                l[c] += w1;
+                split_pair(oc, w0, w1, ph[c].h[j >> 1], pl[c].h[j >> 1]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const Half8 vh = buf.v[b * 2 + h][0][lane], vl = buf.v[b * 2 + h][1][lane];
+#pragma unroll
+                for (int c = 0; c < 2; c++) o[c][b][h] = mfma(vh, ph[c], o[c][b][h]);
+#pragma unroll
+                for (int c = 0; c < 2; c++) o[c][b][h] = mfma(vh, pl[c], o[c][b][h]);
+#pragma unroll
+                for (int c = 0; c < 2; c++) o[c][b][h] = mfma(vl, ph[c], o[c][b][h]);
+            }
+    };
+
+    raw.make(oc, lds.buf[0], sq.len - t_begin * kKvTile, wave, lane);
+    load();
+    lds_barrier();
+    for (int t = t_begin, now = 0; t < t_end; t++, now ^= 1) {
+        raw.make(oc, lds.buf[now ^ 1], sq.len - (t + 1) * kKvTile, wave, lane);
+        load();
+        take(lds.buf[now], t);
+        lds_barrier();
+    }
+
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        l[c] += __shfl_xor(l[c], 16);
+        l[c] += __shfl_xor(l[c], 32);
+        if (g == 0) lds.end.m[wave][col] = m[c] - kLift, lds.end.l[wave][col] = l[c];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&lds.end.o[wave][col][32 * b + 16 * h + 4 * g]) = o[c][b][h];
+        lds_barrier();
+        for (int u = lane >> 5; u < kAttnRows * NB; u += 2) {
+            const int r = u / NB, b = u % NB, d = 32 * b + (lane & 31), fr = row0 + 16 * c + r;
+            const bool ok = 16 * c + r < rows;
+            const float sum = lds.end.o[wave][r][d], mx = lds.end.m[wave][r], den = lds.end.l[wave][r];
+            if (part < 0) {
+                store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, b, NB, sum, den, mx, lane, ok);
+            } else if (ok) {
+                const AttnWork w = attn_work(a);
+                const int64_t at = part * kManyRows + wave * 32 + 16 * c + r;
+                w.outs[at * kDim + d] = sum;
+                if (d == 0) w.tops[at] = make_float2(mx, den);
+            }
+        }
+        lds_barrier();
+    }
+}
+
+// A workgroup a pair of units, the last row tile with the first, and so on
+// inward: the causal ones then have about the same number of tiles.
+template <int BITS, int NB>
+__global__ __launch_bounds__(64 * kManyWaves, kMinWaves<NB>) void k_attn_pairs(AttnArgs a) {
+    __shared__ ManyLds<NB> lds;
+    const int kvh = blockIdx.x % a.kv.kv_heads, pair = blockIdx.x / a.kv.kv_heads, seq = blockIdx.y;
+    const KvSeq sq = kv_seq(a.kv, seq);
+    const int tiles = (sq.n * a.group + kManyRows - 1) / kManyRows;
+    for (int i = 0; i < 2; i++) {
+        const int rt = i ? pair : tiles - 1 - pair;
+        if (i ? pair >= tiles - 1 - pair : rt < pair) return;
+        const Unit u = unit_of<kManyRows>(a, sq, rt);
+        attend_many<BITS, NB>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
+    }
+}
+
+// All units' tiles in a row, cut into equal shares, one a workgroup: however
+// unequal the sequences are, the workgroups end together.  A unit counts
+// kUnitCost tiles more than it has, for its beginning and end.  Every workgroup
+// sums up the units by itself.  The parts of a unit that several workgroups
+// share are numbered (workgroup + unit): along the row each part begins a new
+// workgroup or a new unit.
+constexpr int kUnitCost = UNITCOST;
+template <int BITS, int NB, bool MANY>
+__global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_shares(AttnArgs a) {
+    static_assert(kWaves == kManyWaves);
+    constexpr int kThreads = 64 * kWaves, kEach = kAttnEntries / kThreads, kUnitRows = MANY ? kManyRows : kAttnRows;
+    __shared__ std::conditional_t<MANY, ManyLds<NB>, AttnLds<NB>> lds;
+    __shared__ int before[kAttnEntries + 1];  // cost of a head before each (sequence, row tile)
+    __shared__ int wave_sum[kWaves];
+    const int entries = a.kv.n_seqs * a.row_tiles, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int n[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int e = tid * kEach + i;
+        n[i] = 0;
+        if (e < entries) {
+            const int q = e / a.row_tiles;
+            const Unit u = unit_of<kUnitRows>(a, kv_seq(a.kv, a.kv.rows[q], a.kv.rows[q + 1], a.kv.lens[q]), e % a.row_tiles);
+            n[i] = u.rows ? u.tiles() + kUnitCost : 0;
+        }
+        sum += n[i];
+    }
+    int scan = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(scan, d);
+        if (lane >= d) scan += x;
+    }
+    if (lane == 63) wave_sum[wave] = scan;
+    __syncthreads();
+    int at = scan - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        if (w < wave) at += wave_sum[w];
+        total += wave_sum[w];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        before[tid * kEach + i] = at;
+        at += n[i];
+    }
+    if (tid == kThreads - 1) before[kAttnEntries] = at;
+    __syncthreads();
+    const int64_t all = (int64_t)__builtin_amdgcn_readfirstlane(total) * a.kv.kv_heads;
+    // fewer workgroups where they would have less than a unit's cost
+    const int64_t groups = min((int64_t)a.groups, max((int64_t)1, all / kUnitCost)), b = blockIdx.x;
+    if (b >= groups) return;
+    const int64_t end = (b + 1) * all / groups;
+    int64_t x = b * all / groups;
+    // the entry of x: the last with before[e] * kv_heads <= x
+    int e = 0;
+    if (x < end) {
+        int lo = 0, hi = entries;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((int64_t)before[mid] * a.kv.kv_heads <= x) lo = mid; else hi = mid;
+        }
+        e = lo;
+    }
+    while (x < end) {
+        e = __builtin_amdgcn_readfirstlane(e);
+        const int64_t first = (int64_t)__builtin_amdgcn_readfirstlane(before[e]) * a.kv.kv_heads;
+        const int cost = __builtin_amdgcn_readfirstlane(before[e + 1] - before[e]);
+        const int kvh = cost ? __builtin_amdgcn_readfirstlane((int)((x - first) / cost)) : a.kv.kv_heads;
+        if (kvh >= a.kv.kv_heads) {
+            e++;
+            continue;
+        }
+        const int64_t u0 = first + (int64_t)kvh * cost, u1 = u0 + cost, stop = min(end, u1);
+        // its tiles begin after its cost; a share that ends there has none
+        const int64_t tile0 = u0 + kUnitCost;
+        if (stop > tile0) {
+            const int seq = e / a.row_tiles, rt = e % a.row_tiles;
+            const Unit u = unit_of<kUnitRows>(a, kv_seq(a.kv, seq), rt);
+            const int64_t unit = (int64_t)e * a.kv.kv_heads + kvh;
+            const bool begins = x <= tile0, alone = begins && stop == u1;
+            // the last workgroup whose share begins before u1
+            if (begins && tid == 0) attn_work(a).units[unit] = alone ? make_int2(0, 0) : make_int2((int)b, (int)((u1 * groups - 1) / all));
+            const int t0 = u.t_lo + (int)(max(x, tile0) - tile0), t1 = min(u.t_hi, u.t_lo + (int)(stop - tile0));
+            const int64_t part = alone ? -1 : b + unit;
+            if constexpr (MANY)
+                attend_many<BITS, NB>(a, u, seq, rt, kvh, t0, t1, part, lds);
+            else
+                attend<BITS, NB>(a, u, seq, rt, kvh, t0, t1, part, lds);
+            __syncthreads();
+        }
+        x = stop;
+    }
+}
+
+// The parts of units that workgroups shared: kMergeThreads take `rows` rows at
+// a time, the threads left over share a row's parts.
+constexpr int kMergeThreads = 512;
+template <int NB>
+__global__ __launch_bounds__(kMergeThreads) void k_attn_merge(AttnArgs a, int rows) {
+    constexpr int kDim = 32 * NB;
+    __shared__ float sum[kMergeThreads];
+    const AttnWork w = attn_work(a);
+    const int chunks = a.unit_rows / rows, chunk = blockIdx.x % chunks;
+    const int64_t unit = blockIdx.x / chunks;
+    const int e = (int)(unit / a.kv.kv_heads), kvh = (int)(unit % a.kv.kv_heads), seq = e / a.row_tiles, rt = e % a.row_tiles;
+    const KvSeq sq = kv_seq(a.kv, seq);
+    const int n_rows = min(a.unit_rows, sq.n * a.group - rt * a.unit_rows);
+    if (chunk * rows >= n_rows) return;
+    const int2 wg = w.units[unit];
+    const int n = wg.y - wg.x + 1;
+    if (n <= 1) return;
+    const int tid = threadIdx.x, lane = tid & 63, d = tid % kDim, groups = kMergeThreads / kDim / rows;
+    const int gr = tid / kDim % groups, r = min(chunk * rows + tid / kDim / groups, n_rows - 1);
+    const float2 *top = w.tops + (wg.x + unit) * a.unit_rows + r;
+    const float *out = w.outs + ((wg.x + unit) * a.unit_rows + r) * kDim + d;
+    float m = kNoMax, l = 0.0f, o = 0.0f;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, top[i * a.unit_rows].x);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    for (int i = lane; i < n; i += 64) {
+        const float2 t = top[i * a.unit_rows];
+        l += t.y * __builtin_amdgcn_exp2f(t.x - m);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+#pragma unroll 8
+    for (int i = gr; i < n; i += groups) o += out[(int64_t)i * a.unit_rows * kDim] * __builtin_amdgcn_exp2f(top[i * a.unit_rows].x - m);
+    if (groups > 1) {
+        sum[tid] = o;
+        __syncthreads();
+        if (gr) return;
+        for (int i = 1; i < groups; i++) o += sum[tid + i * kDim];
+    }
+    const int fr = rt * a.unit_rows + r;
+    store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, d / 32, NB, o, l, m, lane,
+              chunk * rows + tid / kDim / groups < n_rows);
 }
 
 }  // namespace
 
 AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int max_len, int window, int n_cu) {
-    AttnPlan p;
-    p.row_tiles = (int)(((int64_t)max_new * group + kAttnRows - 1) / kAttnRows);
-    const int64_t units = (int64_t)n_seqs * kv_heads * p.row_tiles;
+    AttnPlan p{};
+    const int64_t rows = (int64_t)max_new * group;
+    p.unit_rows = rows > kFewRows ? kManyRows : kAttnRows;
+    p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
+    const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads;
     // the tiles of the longest row tile: a window of positions before its first
     // row's, and the rows' own
-    const int own = (kAttnRows - 1) / group + 1;
+    const int own = (p.unit_rows - 1) / group + 1;
     const int64_t seen = window ? std::min<int64_t>(max_len, (int64_t)window + own) : max_len;
-    const int64_t tiles = seen / kKvTile + 2;
-    const int64_t want = std::max<int64_t>(1, (int64_t)n_cu * 4 / units);
-    const int64_t per = std::max<int64_t>(8, (tiles + want - 1) / want);
-    p.splits = (int)((tiles + per - 1) / per);
-    p.split_tiles = (int)per;
-    p.work_bytes = p.splits > 1 ? (uint64_t)units * p.splits * kAttnRows * (32 * nb + 2) * 4 : 0;
+    const int64_t tiles = seen / kKvTile + 2, resident = (int64_t)n_cu * 4 * kMinWaves<2> / kWaves / (nb == 2 ? 1 : 2);
+    const bool many = p.unit_rows == kManyRows;
+    if (tiles > kDirectTiles && entries <= kAttnEntries && (!many || units < resident)) {
+        p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + kUnitCost) / kUnitCost));
+        p.work_bytes = (uint64_t)units * 8 + (uint64_t)(units + p.groups) * p.unit_rows * (8 + 128 * nb);
+    }
     return p;
 }
 
 hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
-    const dim3 grid(a.kv.kv_heads * a.row_tiles * a.splits, a.kv.n_seqs);
+    const bool many = a.unit_rows == kManyRows;
+    const dim3 grid = a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * (many ? (a.row_tiles + 1) / 2 : a.row_tiles), a.kv.n_seqs);
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * kWaves), 0, s, a); };
-    if (bits == 4)
-        nb == 2 ? go(k_attn_split<4, 2>) : go(k_attn_split<4, 4>);
+    auto pick = [&](auto q4_2, auto q4_4, auto q8_2, auto q8_4) {
+        if (bits == 4)
+            nb == 2 ? go(q4_2) : go(q4_4);
+        else
+            nb == 2 ? go(q8_2) : go(q8_4);
+    };
+    if (a.groups && many)
+        pick(k_attn_shares<4, 2, true>, k_attn_shares<4, 4, true>, k_attn_shares<8, 2, true>, k_attn_shares<8, 4, true>);
+    else if (a.groups)
+        pick(k_attn_shares<4, 2, false>, k_attn_shares<4, 4, false>, k_attn_shares<8, 2, false>, k_attn_shares<8, 4, false>);
+    else if (many)
+        pick(k_attn_pairs<4, 2>, k_attn_pairs<4, 4>, k_attn_pairs<8, 2>, k_attn_pairs<8, 4>);
     else
-        nb == 2 ? go(k_attn_split<8, 2>) : go(k_attn_split<8, 4>);
+        pick(k_attn_units<4, 2>, k_attn_units<4, 4>, k_attn_units<8, 2>, k_attn_units<8, 4>);
     return hipGetLastError();
 }
 
 hipError_t launch_attn_merge(hipStream_t s, int nb, const AttnArgs &a) {
-    const dim3 grid(a.kv.kv_heads * a.row_tiles, a.kv.n_seqs);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
+    const int64_t units = (int64_t)a.kv.n_seqs * a.row_tiles * a.kv.kv_heads;
+    // a row a workgroup while the rows are few, else as many as fill it
+    const int rows = units * a.unit_rows <= 2048 ? 1 : kMergeThreads / (32 * nb);
+    const dim3 grid(units * (a.unit_rows / rows));
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kMergeThreads), 0, s, a, rows); };
     nb == 2 ? go(k_attn_merge<2>) : go(k_attn_merge<4>);
     return hipGetLastError();
 }

@@ -64,7 +64,8 @@ struct KvArgs {
     uint8_t *data;
     int kv_heads;
     int page_tiles;  // tiles of a page
-    int64_t n_pages;
+    uint32_t page_inv;  // 2^32 / page_tiles rounded up (its low 32 bits; 0: one tile)
+    int n_pages;
     int n_seqs;
     int max_new;
     int n_rows;
@@ -83,25 +84,44 @@ struct KvSeq {
     bool ok;
 };
 
-__device__ inline KvSeq kv_seq(const KvArgs &a, int s) {
-    const int lo = a.rows[s], hi = a.rows[s + 1];
+__device__ inline KvSeq kv_seq(const KvArgs &a, int lo, int hi, int len) {
     KvSeq q;
     q.r0 = max(0, min(lo, a.n_rows));
     q.n = max(0, min(hi, a.n_rows) - q.r0);
-    q.len = max(0, a.lens[s]);
+    q.len = max(0, len);
     q.first = q.len - q.n;
     q.ok = q.len <= a.max_len && q.n <= a.max_new;
     if (!q.ok) q.n = min(q.n, a.max_new), q.first = 0;
     return q;
 }
 
+// The batch's arrays, which no kernel here writes, as constant memory: a
+// uniform index is then a scalar load, also after the kernel's own stores.
+typedef const int32_t __attribute__((address_space(4))) *KvConst;
+__device__ inline KvConst kv_const(const int32_t *p) { return (KvConst)(uintptr_t)p; }
+
+// Sequence s, the same for all lanes.
+__device__ inline KvSeq kv_seq(const KvArgs &a, int s) {
+    return kv_seq(a, kv_const(a.rows)[s], kv_const(a.rows)[s + 1], kv_const(a.lens)[s]);
+}
+
+// Tile t >= 0 of a sequence: the page of its table, and the tile of that.
+__device__ inline int kv_page_of(const KvArgs &a, int t, int *tile) {
+    // t / page_tiles: the product is at most one too large (t < 2^32)
+    int at = a.page_inv ? (int)__umulhi((uint32_t)t, a.page_inv) : t;
+    if (at * a.page_tiles > t) at--;
+    *tile = t - at * a.page_tiles;
+    return at;
+}
+
 // Tile t of a sequence and head, null where its page is none of the cache's.
 __device__ inline uint8_t *kv_tile(const KvArgs &a, int s, int head, int t, int tile_bytes) {
-    const int at = t / a.page_tiles;
-    if (t < 0 || at >= a.max_pages) return nullptr;
+    int tile;
+    const int at = kv_page_of(a, t, &tile);
+    if (at >= a.max_pages) return nullptr;
     const int page = a.pages[(int64_t)s * a.max_pages + at];
     if (page < 0 || page >= a.n_pages) return nullptr;
-    return a.data + (((int64_t)page * a.kv_heads + head) * a.page_tiles + (t - at * a.page_tiles)) * tile_bytes;
+    return a.data + (((int64_t)page * a.kv_heads + head) * a.page_tiles + tile) * tile_bytes;
 }
 
 // Rotation of pairs (i, i + dim / 2): freq[i] radians a position, cos and sin
@@ -142,19 +162,19 @@ struct AttnArgs {
     int group;      // heads / kv_heads
     float scale;    // of a score, times log2 e
     int window;     // 0: none
-    int row_tiles;  // tiles of rows of a sequence and key/value head
-    int splits;
-    int split_tiles;  // position tiles of a split
-    float *part;      // partial outputs, null: one split
+    int unit_rows;  // rows of a row tile
+    int row_tiles;  // row tiles of a sequence and key/value head
+    int groups;     // workgroups that share all tiles; 0: one a unit, no workspace
+    void *work;
 };
-// What a call launches: how its positions are split, and the workspace that takes.
+// What a call launches, and the workspace that takes.
 struct AttnPlan {
-    int row_tiles, splits, split_tiles;
+    int unit_rows, row_tiles, groups;
     uint64_t work_bytes;
 };
 AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int max_len, int window, int n_cu);
 hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a);
-// After launch_attn, where splits > 1.
+// After launch_attn, where groups > 0.
 hipError_t launch_attn_merge(hipStream_t s, int nb, const AttnArgs &a);
 
 }  // namespace spt
