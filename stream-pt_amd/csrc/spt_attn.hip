@@ -36,7 +36,6 @@ typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kAttnRows = 16;           // rows of a row tile
 #ifndef WAVES
 #define WAVES 8
 #endif
@@ -44,10 +43,16 @@ constexpr int kWaves = WAVES;           // of a workgroup
 constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup sums up
 #ifndef FEW
 #define FEW 32
-#define UNITCOST 8
+#define UNITCOST 16
+#define MANYCOST 2
+#define CHUNK 96
 #endif
 constexpr int kFewRows = FEW;       // up to so many rows of a key/value head: kAttnRows at a time
-constexpr int kDirectTiles = 16;    // a unit of up to so many position tiles is one workgroup's
+constexpr int kChunkTiles = CHUNK;  // 
+#ifndef DIRECT
+#define DIRECT 16
+#endif
+constexpr int kDirectTiles = DIRECT;    // a unit of up to so many position tiles is one workgroup's
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
 constexpr float kLift = 5.0f;       // weights are held times 2^kLift (at most 2^13)
@@ -190,20 +195,17 @@ struct RawTile {
     }
 };
 
-#ifndef AHEAD
-#define AHEAD (NB == 4)
-#endif
 // Whether a tile is loaded while another is taken, and the waves a SIMD that
 // registers have to leave room for.
-template <int BITS, int NB>
-constexpr bool kAhead = AHEAD;
+template <int BITS, int NB, int ROWS>
+constexpr bool kAhead = NB == 4 || (BITS == 4 && ROWS == 8);
 template <int NB>
 #ifndef MINW
 #define MINW 4
 #endif
 constexpr int kMinWaves = NB == 2 ? MINW : 2;
 
-// A unit of work: a row tile (kAttnRows or kManyRows rows) of a sequence and a
+// A unit of work: a row tile (8, 16 or kManyRows rows) of a sequence and a
 // key/value head.  Its rows
 // are tokens [i_first, i_last]; the tiles [t_lo, t_hi) hold what they see.
 struct Unit {
@@ -266,6 +268,48 @@ struct TileWalk {
     }
 };
 
+// The descriptors of tiles t, t + 1, .. of a sequence and head; the table is
+// read a page ahead.
+struct TileRun {
+    KvConst table;
+    const uint8_t *data;
+    uint64_t at;  // of the next tile, from data
+    uint32_t page_bytes, head_bytes, n_pages;
+    int next_page, next_at, max_pages, page_tiles, left, bytes;
+
+    __device__ inline TileRun(const KvArgs &a, int seq, int head, int t, int tile_bytes) {
+        table = kv_const(a.pages) + (int64_t)seq * a.max_pages;
+        data = a.data;
+        page_tiles = a.page_tiles;
+        head_bytes = (uint32_t)head * page_tiles * tile_bytes;
+        page_bytes = (uint32_t)a.kv_heads * page_tiles * tile_bytes;
+        n_pages = (uint32_t)a.n_pages;
+        max_pages = a.max_pages;
+        int tile;
+        next_at = kv_page_of(a, t, &tile);
+        next_page = next_at < max_pages ? table[next_at] : -1;
+        open(tile_bytes);
+        at += (uint32_t)(tile * tile_bytes);
+        left -= tile;
+    }
+    __device__ inline void open(int tile_bytes) {
+        at = (uint64_t)(uint32_t)next_page * page_bytes + head_bytes;
+        bytes = (uint32_t)next_page < n_pages ? tile_bytes : 0;
+        left = page_tiles;
+        next_at++;
+        next_page = next_at < max_pages ? table[next_at] : -1;
+    }
+    // bytes: 0 where there is no page
+    __device__ inline rsrc_t next(int tile_bytes, int *tile_here) {
+        if (left == 0) open(tile_bytes);
+        *tile_here = bytes;
+        const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(data + at), (short)0, bytes, kRsrcWord3);
+        at += (uint32_t)tile_bytes;
+        left--;
+        return r;
+    }
+};
+
 // The workspace: each unit's first and last part, each part's (maximum, sum)
 // of its rows, and its rows' partial outputs.
 struct AttnWork {
@@ -282,17 +326,21 @@ __device__ inline AttnWork attn_work(const AttnArgs &a) {
     return w;
 }
 
-// Sink, division and stores of a row's block of 32 (an element a lane of a
-// half-wave): o / l with the row's maximum m.
-__device__ inline void store_row(const AttnArgs &a, int head, int64_t row, int b, int nb, float o, float l, float m, int lane, bool ok) {
-    float f = 1.0f;
-    if (a.sinks) {
-        const float sink = bias_at(a.sinks, a.sink_type, (uint64_t)head) * 1.44269504088896341f;
-        const float top = fmaxf(m, sink);
-        f = __builtin_amdgcn_exp2f(m - top);
-        l = l * f + __builtin_amdgcn_exp2f(sink - top);
-    }
-    const float v = l == 0.0f ? 0.0f : o * f / l;
+// A head's sink logit (times log2 e; -inf: none).
+__device__ inline float sink_of(const AttnArgs &a, int head) {
+    return a.sinks ? bias_at(a.sinks, a.sink_type, (uint64_t)head) * 1.44269504088896341f : -__builtin_inff();
+}
+
+// What a row's sum of weighted values is multiplied by: one over the sum l of
+// its weights (held times 2^-m) and the sink's.  A row that sees nothing is 0.
+__device__ inline float row_scale(float l, float m, float sink) {
+    const float top = fmaxf(m, sink), f = __builtin_amdgcn_exp2f(m - top);
+    l = l * f + __builtin_amdgcn_exp2f(sink - top);
+    return l == 0.0f ? 0.0f : f / l;
+}
+
+// A row's block of 32 (an element a lane of a half-wave) as output and Q8_0.
+__device__ inline void store_block(const AttnArgs &a, int head, int64_t row, int b, int nb, float v, int lane, bool ok) {
     const int64_t blk = (row * a.heads + head) * nb + b;
     if (ok) a.out[blk * 32 + (lane & 31)] = v;
     if (a.q8) {
@@ -341,13 +389,27 @@ struct Query {
 
 template <int NB>
 struct AttnLds {
-    float o[kWaves][kAttnRows][32 * NB + 4];
-    float m[kWaves][kAttnRows], l[kWaves][kAttnRows];
+    float o[kWaves][16][32 * NB + 4];  // by column
+    float m[kWaves][16], l[kWaves][16], sink[16];
 };
+
+// The value of lane ^ 8, of each row of 16 lanes.
+__device__ inline float other8(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xF, 0xF, false));
+}
+__device__ inline half2v other8(half2v x) {
+    return pk((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__builtin_bit_cast(uint32_t, x), 0x128, 0xF, 0xF, false));
+}
 
 // Tiles [t_begin, t_end) of a unit by the workgroup; the result is the unit's
 // own (part < 0), or that part of it.
-template <int BITS, int NB>
+//
+// ROWS 16: a row a column.  ROWS 8 (up to eight rows, a token of eight heads
+// for instance): columns c and c + 8 are a row's, one multiplied by the hi half of
+// the query or the weights and the other by the lo half, which takes a half
+// to two thirds of the MFMAs.  The two lanes add their halves of a score
+// and take half of the tile's positions each through the softmax.
+template <int BITS, int NB, int ROWS>
 __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, const Unit &un, int seq, int rt, int kvh, int t_begin, int t_end,
                                                              int64_t part, AttnLds<NB> &lds) {
     using T = KvTile<BITS, NB>;
@@ -367,14 +429,23 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
     load(even, p0);
 
     // the row of this lane's column
-    const int flat = rt * kAttnRows + col;
-    const bool row_ok = col < un.rows;
+    constexpr bool kPack = ROWS == 8;
+    const bool upper = kPack && col >= 8;
+    const int flat = rt * ROWS + col % ROWS;
+    const bool row_ok = col % ROWS < un.rows;
     const int tok = row_ok ? flat / a.group : un.i_last, hd = kvh * a.group + (row_ok ? flat % a.group : 0);
     const int pos = sq.first + tok;                   // last position that it sees
     const int from = a.window ? pos - a.window : -1;  // it sees those after this one
 
     Query<NB> q;
+    const float sink = sink_of(a, hd);
     q.load(a, sq.r0 + tok, hd, g);
+    if (kPack) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) q.hi[b].h[i] = upper ? q.lo[b].h[i] : q.hi[b].h[i];
+    }
 
     const Opaque oc;
     f32x4 o[NB][2];
@@ -397,24 +468,35 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
                 Half8 c;
                 raw.keys(oc, h, b, c);
                 f32x4 s = mfma(c, q.hi[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                s = mfma(c, q.lo[b], s);
+                if (!kPack) s = mfma(c, q.lo[b], s);
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[4 * h + i] = raw.scaled(s[i], h, i, b, b ? x[4 * h + i] : oc.zero);
+            }
+        }
+        // the lane's positions begin here, x[0 .. kMine) are theirs
+        constexpr int kMine = kPack ? 4 : 8;
+        const int mine = p0 + 8 * g + (upper ? 4 : 0);
+        if (kPack) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float keep = upper ? x[4 + i] : x[i], give = upper ? x[i] : x[4 + i];
+                x[i] = keep + other8(give);
             }
         }
         if (!whole) {
             asm volatile("");  // a branch: the whole tiles, nearly all, do without
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int p = p0 + 8 * g + j;
+            for (int j = 0; j < kMine; j++) {
+                const int p = mine + j;
                 x[j] = p <= pos && p > from ? x[j] : -__builtin_inff();
             }
             if (p0 + kKvTile > sq.len) raw.clear_values(sq.len - p0 - 8 * g);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) top = fmaxf(top, x[j]);
+        for (int j = 0; j < kMine; j++) top = fmaxf(top, x[j]);
         top *= q.mul;
         if (__any(top > m + kSlack)) {
+            if (kPack) top = fmaxf(top, other8(top));
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             const float nm = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - nm);
@@ -426,11 +508,20 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
         Half8 ph, pl;
         const float back = kLift - m;
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
+        for (int j = 0; j < kMine; j += 2) {
             const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], q.mul, back)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j + 1], q.mul, back));
             l += w0;
             l += w1;
             split_pair(oc, w0, w1, ph.h[j >> 1], pl.h[j >> 1]);
+        }
+        if (kPack) {
+            // the hi column's weights of all positions, and the lo column's
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const half2v got = other8(upper ? ph.h[i] : pl.h[i]);
+                ph.h[2 + i] = upper ? pl.h[i] : got;
+                ph.h[i] = upper ? got : ph.h[i];
+            }
         }
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -439,11 +530,11 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
                 Half8 vh, vl;
                 raw.values(oc, b, h, vh, vl);
                 o[b][h] = mfma(vh, ph, o[b][h]);
-                o[b][h] = mfma(vh, pl, o[b][h]);
+                if (!kPack) o[b][h] = mfma(vh, pl, o[b][h]);
                 o[b][h] = mfma(vl, ph, o[b][h]);
             }
     };
-    if (kAhead<BITS, NB>) {
+    if (kAhead<BITS, NB, ROWS>) {
         // two tiles in registers, one being loaded while the other is taken
         RawTile<BITS, NB> odd;
         while (t < t_end) {
@@ -469,9 +560,10 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
     }
 
     // the waves' parts, on the largest maximum
+    if (kPack) l += other8(l);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) lds.m[wave][col] = m, lds.l[wave][col] = l;
+    if (g == 0) lds.m[wave][col] = m, lds.l[wave][col] = l, lds.sink[col] = sink;
     __syncthreads();
     float top = lds.m[0][col];
 #pragma unroll
@@ -483,7 +575,7 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
         for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&lds.o[wave][col][32 * b + 16 * h + 4 * g]) = o[b][h] * f;
     __syncthreads();
     // a half-wave takes a block of a row
-    for (int u = wave * 2 + (lane >> 5); u < kAttnRows * NB; u += 2 * kWaves) {
+    for (int u = wave * 2 + (lane >> 5); u < ROWS * NB; u += 2 * kWaves) {
         const int r = u / NB, b = u % NB, d = 32 * b + (lane & 31);
         float mx = lds.m[0][r], sum = 0.0f, den = 0.0f;
 #pragma unroll
@@ -492,27 +584,28 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
         for (int w = 0; w < kWaves; w++) {
             den += lds.l[w][r] * __builtin_amdgcn_exp2f(lds.m[w][r] - mx);
             sum += lds.o[w][r][d];
+            if (kPack) sum += lds.o[w][r + 8][d];
         }
         mx -= kLift;  // weights are 2^kLift too large, the sink is not
-        const int fr = rt * kAttnRows + r;
+        const int fr = rt * ROWS + r;
         const bool ok = r < un.rows;
         if (part < 0) {
-            store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, b, NB, sum, den, mx, lane, ok);
+            store_block(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, b, NB, sum * row_scale(den, mx, lds.sink[r]), lane, ok);
         } else if (ok) {
             const AttnWork w = attn_work(a);
-            w.outs[(part * kAttnRows + r) * kDim + d] = sum;
-            if (d == 0) w.tops[part * kAttnRows + r] = make_float2(mx, den);
+            w.outs[(part * ROWS + r) * kDim + d] = sum;
+            if (d == 0) w.tops[part * ROWS + r] = make_float2(mx, den);
         }
     }
 }
 
 // A workgroup a unit.
-template <int BITS, int NB>
+template <int BITS, int NB, int ROWS>
 __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_units(AttnArgs a) {
     __shared__ AttnLds<NB> lds;
     const int kvh = blockIdx.x % a.kv.kv_heads, rt = blockIdx.x / a.kv.kv_heads, seq = blockIdx.y;
-    const Unit u = unit_of<kAttnRows>(a, kv_seq(a.kv, seq), rt);
-    if (u.rows) attend<BITS, NB>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
+    const Unit u = unit_of<ROWS>(a, kv_seq(a.kv, seq), rt);
+    if (u.rows) attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
 }
 
 // Rows many at a time: a workgroup's 8 waves have 32 rows each (two columns of
@@ -521,7 +614,11 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_units(AttnA
 // next is made in the other and the bytes of the one after it are on their
 // way.  Each wave makes an eighth of a tile: a unit is a key or value operand of
 // one MFMA, 1 KB or twice 1 KB.
-constexpr int kManyWaves = 8, kManyRows = 32 * kManyWaves;
+#ifndef MANYW
+#define MANYW 8
+#define MMINW 2
+#endif
+constexpr int kManyWaves = MANYW, kManyRows = 32 * kManyWaves;
 
 template <int NB>
 union ManyLds {
@@ -530,16 +627,13 @@ union ManyLds {
         Half8 v[2 * NB][2][64];  // [b][h][hi, lo][lane]
         u32x4 ks[4 * NB];        // scales as they are stored
     } buf[2];
-    struct {
-        float o[kManyWaves][kAttnRows][32 * NB + 4];
-        float m[kManyWaves][kAttnRows], l[kManyWaves][kAttnRows];
-    } end;
+    float o[kManyWaves][16][32 * NB + 4];
 };
 
 // A wave's part of a tile: NB / 2 units of keys (waves 0 to 3) or values.
 template <int BITS, int NB>
 struct ManyPart {
-    static constexpr int kUnits = NB / 2;
+    static constexpr int kHalf = kManyWaves / 2, kUnits = 2 * NB / kHalf;  // waves for keys, units of each
     uint2 c[kUnits];
     u32x4 d[kUnits];  // values: scales of eight positions; keys: all scales, by the first lanes
     bool ok;
@@ -552,8 +646,8 @@ struct ManyPart {
         ok = page_ok;
 #pragma unroll
         for (int j = 0; j < kUnits; j++) {
-            const int u = (wave & 3) * kUnits + j;
-            if (wave < 4) {
+            const int u = wave % kHalf * kUnits + j;
+            if (wave < kHalf) {
                 const int t = u / NB, b = u % NB;
                 if (BITS == 4)
                     c[j].x = __builtin_amdgcn_raw_buffer_load_b32(tile, lane * 16, (b >> 1) * 1024 + t * 8 + (b & 1) * 4, 0);
@@ -572,8 +666,8 @@ struct ManyPart {
     __device__ inline void make(const Opaque &o, typename ManyLds<NB>::Buffer &buf, int left, int wave, int lane) {
 #pragma unroll
         for (int j = 0; j < kUnits; j++) {
-            const int u = (wave & 3) * kUnits + j;
-            if (wave < 4) {
+            const int u = wave % kHalf * kUnits + j;
+            if (wave < kHalf) {
                 Half8 k;
                 if (BITS == 4)
                     q4_key(o, c[j].x, k);
@@ -585,8 +679,8 @@ struct ManyPart {
             } else {
                 Half8 v, hi, lo;
                 if (BITS == 4) {
-                    q4_value(o, c[j].x, c[j].y, 0, v);
-                    if (u & 1) q4_value(o, c[j].x, c[j].y, 1, v);
+                    const int down = 4 * (u & 1);  // the upper nibbles moved to the lower's place
+                    q4_value(o, c[j].x >> down, c[j].y >> down, 0, v);
                 } else {
                     q8_codes(c[j].x, c[j].y, v);
                 }
@@ -607,12 +701,12 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
     const KvSeq &sq = un.sq;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    TileWalk walk(a.kv, seq, kvh, t_begin, 1, T::kBytes);
+    TileRun run(a.kv, seq, kvh, t_begin, T::kBytes);
     ManyPart<BITS, NB> raw;
     auto load = [&]() __attribute__((always_inline)) {
-        const TileWalk::Place p = walk.next();
-        const bool ok = walk.ok(p);
-        raw.load(__builtin_amdgcn_make_buffer_rsrc(a.kv.data + walk.offset(p), (short)0, ok ? T::kBytes : 0, kRsrcWord3), ok, wave, lane);
+        int bytes;
+        const rsrc_t tile = run.next(T::kBytes, &bytes);
+        raw.load(tile, bytes != 0, wave, lane);
     };
     load();
 
@@ -621,6 +715,7 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
     const int i0 = row0 / a.group, i1 = (row0 + min(rows, 32) - 1) / a.group;  // its tokens
     const int pos0 = sq.first + i0, pos1 = sq.first + i1;
     int pos[2], from[2];
+    float sink[2];
     Query<NB> q[2];
     f32x4 o[2][NB][2];
     float m[2] = {kNoMax, kNoMax}, l[2];
@@ -631,6 +726,7 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
         const int tok = ok ? (row0 + r) / a.group : un.i_last, hd = kvh * a.group + (ok ? (row0 + r) % a.group : 0);
         pos[c] = sq.first + tok;
         from[c] = a.window ? pos[c] - a.window : -1;
+        sink[c] = sink_of(a, hd);
         q[c].load(a, sq.r0 + tok, hd, g);
         l[c] = sq.ok ? 0.0f : __builtin_nanf("");
 #pragma unroll
@@ -638,11 +734,15 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
     }
     const Opaque oc;
 
+    // The tiles that any of this wave's rows sees (the others are made for the
+    // other waves), and those of them that all its rows see whole.
+    const int w_begin = a.window ? max(0, pos0 - a.window + 1) / kKvTile : 0;
+    const int w_end = rows <= 0 || pos1 < 0 ? 0 : pos1 / kKvTile + 1;
+    const int whole_begin = a.window ? (max(0, pos1 - a.window + 1) + kKvTile - 1) / kKvTile : 0;
+    const int whole_end = (max(-1, pos0) + 1) / kKvTile;
     auto take = [&](const typename ManyLds<NB>::Buffer &buf, int t) __attribute__((always_inline)) {
+        if (t < w_begin || t >= w_end) return;
         const int p0 = t * kKvTile;
-        // nothing here is for this wave's rows
-        if (rows <= 0 || p0 > pos1 || (a.window && p0 + kKvTile - 1 <= pos0 - a.window)) return;
-        const bool whole = p0 + kKvTile - 1 <= pos0 && (!a.window || p0 > pos1 - a.window);
         u32x4 ks[NB];
 #pragma unroll
         for (int i = 0; i < NB; i++) ks[i] = buf.ks[g * NB + i];
@@ -663,7 +763,7 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
                     }
                 }
             }
-        if (!whole) {
+        if (t < whole_begin || t >= whole_end) {
             asm volatile("");
 #pragma unroll
             for (int c = 0; c < 2; c++)
@@ -723,34 +823,48 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
     raw.make(oc, lds.buf[0], sq.len - t_begin * kKvTile, wave, lane);
     load();
     lds_barrier();
-    for (int t = t_begin, now = 0; t < t_end; t++, now ^= 1) {
+    auto step = [&](int t, int now) __attribute__((always_inline)) {
         raw.make(oc, lds.buf[now ^ 1], sq.len - (t + 1) * kKvTile, wave, lane);
         load();
         take(lds.buf[now], t);
         lds_barrier();
+    };
+    for (int t = t_begin; t < t_end; t += 2) {
+        step(t, 0);
+        if (t + 1 < t_end) step(t + 1, 1);
     }
 
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         l[c] += __shfl_xor(l[c], 16);
         l[c] += __shfl_xor(l[c], 32);
-        if (g == 0) lds.end.m[wave][col] = m[c] - kLift, lds.end.l[wave][col] = l[c];
+        m[c] -= kLift;  // weights are 2^kLift too large, the sink is not
+        const AttnWork w = attn_work(a);
+        const int64_t at = part * kManyRows + wave * 32 + 16 * c;  // the part's rows
+        const float f = part < 0 ? row_scale(l[c], m[c], sink[c]) : 1.0f;
+        if (part >= 0 && g == 0 && 16 * c + col < rows) w.tops[at + col] = make_float2(m[c], l[c]);
+        // through LDS, so that a row's output is stored by consecutive lanes
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&lds.end.o[wave][col][32 * b + 16 * h + 4 * g]) = o[c][b][h];
+            for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&lds.o[wave][col][32 * b + 16 * h + 4 * g]) = o[c][b][h] * f;
         lds_barrier();
-        for (int u = lane >> 5; u < kAttnRows * NB; u += 2) {
-            const int r = u / NB, b = u % NB, d = 32 * b + (lane & 31), fr = row0 + 16 * c + r;
-            const bool ok = 16 * c + r < rows;
-            const float sum = lds.end.o[wave][r][d], mx = lds.end.m[wave][r], den = lds.end.l[wave][r];
-            if (part < 0) {
-                store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, b, NB, sum, den, mx, lane, ok);
-            } else if (ok) {
-                const AttnWork w = attn_work(a);
-                const int64_t at = part * kManyRows + wave * 32 + 16 * c + r;
-                w.outs[at * kDim + d] = sum;
-                if (d == 0) w.tops[at] = make_float2(mx, den);
+        constexpr int kQuads = kDim / 4;
+#pragma unroll 4
+        for (int u = lane; u < 16 * kQuads; u += 64) {
+            const int r = u / kQuads, d = u % kQuads * 4, fr = row0 + 16 * c + r;
+            if (16 * c + r >= rows) continue;
+            float *to = part < 0 ? a.out + ((int64_t)(sq.r0 + fr / a.group) * a.heads + kvh * a.group + fr % a.group) * kDim : w.outs + (at + r) * kDim;
+            *reinterpret_cast<f32x4 *>(to + d) = *reinterpret_cast<const f32x4 *>(&lds.o[wave][r][d]);
+        }
+        if (a.q8 && part < 0) {
+            for (int u = lane >> 5; u < 16 * NB; u += 2) {
+                const int r = u / NB, b = u % NB, fr = row0 + 16 * c + r;
+                uint16_t dh;
+                const int x = q8_quantize_half(lds.o[wave][r][32 * b + (lane & 31)], lane, &dh);
+                if (16 * c + r < rows)
+                    write_q8_lane(x, dh, lane & 31, (size_t)(((sq.r0 + fr / a.group) * (int64_t)a.heads + kvh * a.group + fr % a.group) * NB + b),
+                                  nullptr, nullptr, nullptr, a.q8);
             }
         }
         lds_barrier();
@@ -760,7 +874,7 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
 // A workgroup a pair of units, the last row tile with the first, and so on
 // inward: the causal ones then have about the same number of tiles.
 template <int BITS, int NB>
-__global__ __launch_bounds__(64 * kManyWaves, kMinWaves<NB>) void k_attn_pairs(AttnArgs a) {
+__global__ __launch_bounds__(64 * kManyWaves, NB == 2 ? MMINW : 2) void k_attn_pairs(AttnArgs a) {
     __shared__ ManyLds<NB> lds;
     const int kvh = blockIdx.x % a.kv.kv_heads, pair = blockIdx.x / a.kv.kv_heads, seq = blockIdx.y;
     const KvSeq sq = kv_seq(a.kv, seq);
@@ -779,14 +893,15 @@ __global__ __launch_bounds__(64 * kManyWaves, kMinWaves<NB>) void k_attn_pairs(A
 // sums up the units by itself.  The parts of a unit that several workgroups
 // share are numbered (workgroup + unit): along the row each part begins a new
 // workgroup or a new unit.
-constexpr int kUnitCost = UNITCOST;
-template <int BITS, int NB, bool MANY>
-__global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_shares(AttnArgs a) {
-    static_assert(kWaves == kManyWaves);
-    constexpr int kThreads = 64 * kWaves, kEach = kAttnEntries / kThreads, kUnitRows = MANY ? kManyRows : kAttnRows;
+constexpr int kUnitCost = UNITCOST, kManyCost = MANYCOST;
+template <int BITS, int NB, int ROWS>
+__global__ __launch_bounds__(64 * (ROWS == kManyRows ? kManyWaves : kWaves), NB == 2 ? (ROWS == kManyRows ? MMINW : kMinWaves<2>) : 2) void k_attn_shares(AttnArgs a) {
+    constexpr bool MANY = ROWS == kManyRows;
+    constexpr int kCost = MANY ? kManyCost : kUnitCost;
+    constexpr int kNWaves = MANY ? kManyWaves : kWaves, kThreads = 64 * kNWaves, kEach = kAttnEntries / kThreads;
     __shared__ std::conditional_t<MANY, ManyLds<NB>, AttnLds<NB>> lds;
     __shared__ int before[kAttnEntries + 1];  // cost of a head before each (sequence, row tile)
-    __shared__ int wave_sum[kWaves];
+    __shared__ int wave_sum[kNWaves];
     const int entries = a.kv.n_seqs * a.row_tiles, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int n[kEach], sum = 0;
 #pragma unroll
@@ -795,8 +910,8 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_shares(Attn
         n[i] = 0;
         if (e < entries) {
             const int q = e / a.row_tiles;
-            const Unit u = unit_of<kUnitRows>(a, kv_seq(a.kv, a.kv.rows[q], a.kv.rows[q + 1], a.kv.lens[q]), e % a.row_tiles);
-            n[i] = u.rows ? u.tiles() + kUnitCost : 0;
+            const Unit u = unit_of<ROWS>(a, kv_seq(a.kv, a.kv.rows[q], a.kv.rows[q + 1], a.kv.lens[q]), e % a.row_tiles);
+            n[i] = u.rows ? u.tiles() + kCost : 0;
         }
         sum += n[i];
     }
@@ -810,7 +925,7 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_shares(Attn
     __syncthreads();
     int at = scan - sum, total = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
+    for (int w = 0; w < kNWaves; w++) {
         if (w < wave) at += wave_sum[w];
         total += wave_sum[w];
     }
@@ -823,7 +938,7 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_shares(Attn
     __syncthreads();
     const int64_t all = (int64_t)__builtin_amdgcn_readfirstlane(total) * a.kv.kv_heads;
     // fewer workgroups where they would have less than a unit's cost
-    const int64_t groups = min((int64_t)a.groups, max((int64_t)1, all / kUnitCost)), b = blockIdx.x;
+    const int64_t groups = min((int64_t)a.groups, max((int64_t)1, all / kCost)), b = blockIdx.x;
     if (b >= groups) return;
     const int64_t end = (b + 1) * all / groups;
     int64_t x = b * all / groups;
@@ -848,10 +963,10 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_shares(Attn
         }
         const int64_t u0 = first + (int64_t)kvh * cost, u1 = u0 + cost, stop = min(end, u1);
         // its tiles begin after its cost; a share that ends there has none
-        const int64_t tile0 = u0 + kUnitCost;
+        const int64_t tile0 = u0 + kCost;
         if (stop > tile0) {
             const int seq = e / a.row_tiles, rt = e % a.row_tiles;
-            const Unit u = unit_of<kUnitRows>(a, kv_seq(a.kv, seq), rt);
+            const Unit u = unit_of<ROWS>(a, kv_seq(a.kv, seq), rt);
             const int64_t unit = (int64_t)e * a.kv.kv_heads + kvh;
             const bool begins = x <= tile0, alone = begins && stop == u1;
             // the last workgroup whose share begins before u1
@@ -861,7 +976,7 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_shares(Attn
             if constexpr (MANY)
                 attend_many<BITS, NB>(a, u, seq, rt, kvh, t0, t1, part, lds);
             else
-                attend<BITS, NB>(a, u, seq, rt, kvh, t0, t1, part, lds);
+                attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, t0, t1, part, lds);
             __syncthreads();
         }
         x = stop;
@@ -908,8 +1023,9 @@ __global__ __launch_bounds__(kMergeThreads) void k_attn_merge(AttnArgs a, int ro
         for (int i = 1; i < groups; i++) o += sum[tid + i * kDim];
     }
     const int fr = rt * a.unit_rows + r;
-    store_row(a, kvh * a.group + fr % a.group, sq.r0 + fr / a.group, d / 32, NB, o, l, m, lane,
-              chunk * rows + tid / kDim / groups < n_rows);
+    const int head = kvh * a.group + fr % a.group;
+    store_block(a, head, sq.r0 + fr / a.group, d / 32, NB, o * row_scale(l, m, sink_of(a, head)), lane,
+                chunk * rows + tid / kDim / groups < n_rows);
 }
 
 }  // namespace
@@ -917,17 +1033,27 @@ __global__ __launch_bounds__(kMergeThreads) void k_attn_merge(AttnArgs a, int ro
 AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int max_len, int window, int n_cu) {
     AttnPlan p{};
     const int64_t rows = (int64_t)max_new * group;
-    p.unit_rows = rows > kFewRows ? kManyRows : kAttnRows;
-    p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
-    const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads;
-    // the tiles of the longest row tile: a window of positions before its first
+    // the position tiles of a unit of so many rows: a window before its first
     // row's, and the rows' own
-    const int own = (p.unit_rows - 1) / group + 1;
-    const int64_t seen = window ? std::min<int64_t>(max_len, (int64_t)window + own) : max_len;
-    const int64_t tiles = seen / kKvTile + 2, resident = (int64_t)n_cu * 4 * kMinWaves<2> / kWaves / (nb == 2 ? 1 : 2);
+    auto tiles_of = [&](int unit_rows) {
+        const int64_t own = (unit_rows - 1) / group + 1;
+        return (window ? std::min<int64_t>(max_len, window + own) : max_len) / kKvTile + 2;
+    };
+    auto units_of = [&](int unit_rows) { return (int64_t)n_seqs * kv_heads * ((rows + unit_rows - 1) / unit_rows); };
+    if (rows <= 8)
+        p.unit_rows = 8;
+    else if (rows <= kFewRows || (units_of(16) <= n_cu && tiles_of(16) <= kChunkTiles))
+        p.unit_rows = 16;
+    else
+        p.unit_rows = kManyRows;
     const bool many = p.unit_rows == kManyRows;
-    if (tiles > kDirectTiles && entries <= kAttnEntries && (!many || units < resident)) {
-        p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + kUnitCost) / kUnitCost));
+    p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
+    const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
+    const int64_t resident = many ? (int64_t)n_cu * 4 * (nb == 2 ? MMINW : 2) / kManyWaves : (int64_t)n_cu * 4 * (nb == 2 ? kMinWaves<2> : 2) / kWaves;
+    const bool direct = many ? units >= resident : rows > kFewRows || tiles <= kDirectTiles;
+    if (!direct && entries <= kAttnEntries) {
+        const int64_t cost = many ? kManyCost : kUnitCost;
+        p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + cost) / cost));
         p.work_bytes = (uint64_t)units * 8 + (uint64_t)(units + p.groups) * p.unit_rows * (8 + 128 * nb);
     }
     return p;
@@ -936,21 +1062,19 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
 hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
     const bool many = a.unit_rows == kManyRows;
     const dim3 grid = a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * (many ? (a.row_tiles + 1) / 2 : a.row_tiles), a.kv.n_seqs);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * kWaves), 0, s, a); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, a); };
     auto pick = [&](auto q4_2, auto q4_4, auto q8_2, auto q8_4) {
         if (bits == 4)
             nb == 2 ? go(q4_2) : go(q4_4);
         else
             nb == 2 ? go(q8_2) : go(q8_4);
     };
-    if (a.groups && many)
-        pick(k_attn_shares<4, 2, true>, k_attn_shares<4, 4, true>, k_attn_shares<8, 2, true>, k_attn_shares<8, 4, true>);
-    else if (a.groups)
-        pick(k_attn_shares<4, 2, false>, k_attn_shares<4, 4, false>, k_attn_shares<8, 2, false>, k_attn_shares<8, 4, false>);
-    else if (many)
-        pick(k_attn_pairs<4, 2>, k_attn_pairs<4, 4>, k_attn_pairs<8, 2>, k_attn_pairs<8, 4>);
+#define SPT_PICK(kernel, ...) pick(kernel<4, 2, ##__VA_ARGS__>, kernel<4, 4, ##__VA_ARGS__>, kernel<8, 2, ##__VA_ARGS__>, kernel<8, 4, ##__VA_ARGS__>)
+    if (a.groups)
+        many ? SPT_PICK(k_attn_shares, kManyRows) : a.unit_rows == 8 ? SPT_PICK(k_attn_shares, 8) : SPT_PICK(k_attn_shares, 16);
     else
-        pick(k_attn_units<4, 2>, k_attn_units<4, 4>, k_attn_units<8, 2>, k_attn_units<8, 4>);
+        many ? SPT_PICK(k_attn_pairs) : a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8) : SPT_PICK(k_attn_units, 16);
+#undef SPT_PICK
     return hipGetLastError();
 }
 
