@@ -13,14 +13,21 @@
 // lo * lo being below 2^-22 of the product.  (Scaling the weights by each
 // block's d instead takes as many instructions, and leaves fp16's range.)
 //
-// k_attn_split, rows 16 at a time (a column of the MFMA each; the group's
-// heads of one or more tokens): a wave takes tiles of 32 positions in turn
-// and makes their operands in its registers, scores of a tile are its D
-// registers, and those are the B operand of the product with the values.  The
+// Few rows (attend: 8 or 16 of a key/value head at a time, a column of the MFMA
+// each or two): the workgroup's waves take tiles of 32 positions in turn and
+// make their operands in registers; a tile's scores are its D registers, and
+// those are the B operand of the product with the values.  Many rows
+// (attend_many: 256 at a time): operands are made once a workgroup in LDS.  The
 // running maximum is one number a row, raised only when a score passes it by
-// kSlack (weights up to 2^kSlack fit fp16 beside the scale), so most tiles need
-// no exchange between lanes and no rescaling.  The waves' parts meet in LDS;
-// where the rows are few, splits of the positions meet in k_attn_merge.
+// kSlack (weights up to 2^kSlack fit fp16 beside the lift), so most tiles need
+// no exchange between lanes and no rescaling.
+//
+// What bounds it: the vector instructions that unpack values and form weights,
+// and the MFMAs, which overlap with them in part only (16 MFMAs and 64 FMAs of
+// two waves on a SIMD, one wave each: 463 cycles, 319 and 322 alone).  One
+// token over 1,048,576 positions of 8 heads of 64 (604 MB) takes 144 us, 4.2 TB/s;
+// over 131,071, 28.4 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times that
+// with the halves): 110 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,23 +43,21 @@ typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-#ifndef WAVES
-#define WAVES 8
-#endif
-constexpr int kWaves = WAVES;           // of a workgroup
-constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup sums up
-#ifndef FEW
-#define FEW 32
-#define UNITCOST 16
-#define MANYCOST 2
-#define CHUNK 96
-#endif
-constexpr int kFewRows = FEW;       // up to so many rows of a key/value head: kAttnRows at a time
-constexpr int kChunkTiles = CHUNK;  // 
-#ifndef DIRECT
-#define DIRECT 16
-#endif
-constexpr int kDirectTiles = DIRECT;    // a unit of up to so many position tiles is one workgroup's
+constexpr int kWaves = 8;  // of a workgroup (few rows)
+// Launches, by what the batch's bounds allow (us, one token of 64 heads on 8 of 64
+// unless said otherwise):
+//   rows of a key/value head: up to 8, two columns a row (an 8-head token, 64 ragged
+//   sequences up to 8,192: 59, a column a row 70); up to kFewRows, 16 at a
+//   time; more, 256 at a time, except where 16 at a time are at most a workgroup a
+//   compute unit and kChunkTiles tiles long (32 tokens over 2,049 positions: 13, 256
+//   at a time 33);
+//   a workgroup a unit (a row tile of a sequence and head) up to kDirectTiles position
+//   tiles, and further, up to kWideTiles, in proportion to the units while they do
+//   not fill the compute units (1 sequence of 2,048: 11.5, shares 12.8; of 4,096:
+//   18.3, 13.2; 64 ragged ones up to 4,096: 31, 40; up to 16,384: 104, 97); beyond,
+//   equal shares of all tiles and a second launch.
+constexpr int kFewRows = 32, kChunkTiles = 96, kDirectTiles = 72, kWideTiles = 300;
+constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup of the shares sums up
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
 constexpr float kLift = 5.0f;       // weights are held times 2^kLift (at most 2^13)
@@ -64,9 +69,6 @@ union Half8 {
 
 __device__ inline half2v pk(uint32_t w) { return __builtin_bit_cast(half2v, w); }
 
-// Codes of eight positions or dims as fp16 pairs.  Q4_0: w's low nibbles (or
-// high) of bytes 0 and 2, then 1 and 3, into the low mantissa bits of 1024
-// (or 16 places higher, 64 + n after the multiply by 1/16).
 // Constants that the compiler does not see through: with them it makes one
 // v_and_or_b32 of the mask and the or, and one mixed-precision FMA of a
 // conversion and a product or sum, where it would fold known ones apart.
@@ -82,6 +84,9 @@ struct Opaque {
     }
 };
 
+// Codes as fp16 pairs.  Q4_0: the low (or high) nibbles of bytes 0 and 2 into the
+// low mantissa bits of 1024 (or four places higher: 64 + n after the multiply by
+// 1/16).
 __device__ inline half2v q4_low(const Opaque &o, uint32_t w) { return pk((w & o.low) | o.k1024) + (half2v)(_Float16)-1032.0f; }
 __device__ inline half2v q4_high(const Opaque &o, uint32_t w) {
     return __builtin_elementwise_fma(pk((w & o.high) | o.k1024), (half2v)(_Float16)0.0625f, (half2v)(_Float16)-72.0f);
@@ -200,10 +205,7 @@ struct RawTile {
 template <int BITS, int NB, int ROWS>
 constexpr bool kAhead = NB == 4 || (BITS == 4 && ROWS == 8);
 template <int NB>
-#ifndef MINW
-#define MINW 4
-#endif
-constexpr int kMinWaves = NB == 2 ? MINW : 2;
+constexpr int kMinWaves = NB == 2 ? 4 : 2;
 
 // A unit of work: a row tile (8, 16 or kManyRows rows) of a sequence and a
 // key/value head.  Its rows
@@ -614,11 +616,8 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_units(AttnA
 // next is made in the other and the bytes of the one after it are on their
 // way.  Each wave makes an eighth of a tile: a unit is a key or value operand of
 // one MFMA, 1 KB or twice 1 KB.
-#ifndef MANYW
-#define MANYW 8
-#define MMINW 2
-#endif
-constexpr int kManyWaves = MANYW, kManyRows = 32 * kManyWaves;
+constexpr int kManyWaves = 8, kManyRows = 32 * kManyWaves;
+static_assert(kManyWaves == kWaves, "one launch shape");
 
 template <int NB>
 union ManyLds {
@@ -874,7 +873,7 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
 // A workgroup a pair of units, the last row tile with the first, and so on
 // inward: the causal ones then have about the same number of tiles.
 template <int BITS, int NB>
-__global__ __launch_bounds__(64 * kManyWaves, NB == 2 ? MMINW : 2) void k_attn_pairs(AttnArgs a) {
+__global__ __launch_bounds__(64 * kManyWaves, 2) void k_attn_pairs(AttnArgs a) {
     __shared__ ManyLds<NB> lds;
     const int kvh = blockIdx.x % a.kv.kv_heads, pair = blockIdx.x / a.kv.kv_heads, seq = blockIdx.y;
     const KvSeq sq = kv_seq(a.kv, seq);
@@ -893,15 +892,15 @@ __global__ __launch_bounds__(64 * kManyWaves, NB == 2 ? MMINW : 2) void k_attn_p
 // sums up the units by itself.  The parts of a unit that several workgroups
 // share are numbered (workgroup + unit): along the row each part begins a new
 // workgroup or a new unit.
-constexpr int kUnitCost = UNITCOST, kManyCost = MANYCOST;
+constexpr int kUnitCost = 16, kManyCost = 2;
 template <int BITS, int NB, int ROWS>
-__global__ __launch_bounds__(64 * (ROWS == kManyRows ? kManyWaves : kWaves), NB == 2 ? (ROWS == kManyRows ? MMINW : kMinWaves<2>) : 2) void k_attn_shares(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, ROWS == kManyRows ? 2 : kMinWaves<NB>) void k_attn_shares(AttnArgs a) {
     constexpr bool MANY = ROWS == kManyRows;
     constexpr int kCost = MANY ? kManyCost : kUnitCost;
-    constexpr int kNWaves = MANY ? kManyWaves : kWaves, kThreads = 64 * kNWaves, kEach = kAttnEntries / kThreads;
+    constexpr int kThreads = 64 * kWaves, kEach = kAttnEntries / kThreads;
     __shared__ std::conditional_t<MANY, ManyLds<NB>, AttnLds<NB>> lds;
     __shared__ int before[kAttnEntries + 1];  // cost of a head before each (sequence, row tile)
-    __shared__ int wave_sum[kNWaves];
+    __shared__ int wave_sum[kWaves];
     const int entries = a.kv.n_seqs * a.row_tiles, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int n[kEach], sum = 0;
 #pragma unroll
@@ -925,7 +924,7 @@ __global__ __launch_bounds__(64 * (ROWS == kManyRows ? kManyWaves : kWaves), NB 
     __syncthreads();
     int at = scan - sum, total = 0;
 #pragma unroll
-    for (int w = 0; w < kNWaves; w++) {
+    for (int w = 0; w < kWaves; w++) {
         if (w < wave) at += wave_sum[w];
         total += wave_sum[w];
     }
@@ -1049,8 +1048,8 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
     const bool many = p.unit_rows == kManyRows;
     p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
     const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
-    const int64_t resident = many ? (int64_t)n_cu * 4 * (nb == 2 ? MMINW : 2) / kManyWaves : (int64_t)n_cu * 4 * (nb == 2 ? kMinWaves<2> : 2) / kWaves;
-    const bool direct = many ? units >= resident : rows > kFewRows || tiles <= kDirectTiles;
+    const int64_t resident = (int64_t)n_cu * 4 * (many || nb == 4 ? 2 : kMinWaves<2>) / kWaves;  // workgroups at once
+    const bool direct = many ? units >= resident : rows > kFewRows || tiles <= std::max<int64_t>(kDirectTiles, std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu));
     if (!direct && entries <= kAttnEntries) {
         const int64_t cost = many ? kManyCost : kUnitCost;
         p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + cost) / cost));
@@ -1062,7 +1061,7 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
 hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
     const bool many = a.unit_rows == kManyRows;
     const dim3 grid = a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * (many ? (a.row_tiles + 1) / 2 : a.row_tiles), a.kv.n_seqs);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, a); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * kWaves), 0, s, a); };
     auto pick = [&](auto q4_2, auto q4_4, auto q8_2, auto q8_4) {
         if (bits == 4)
             nb == 2 ? go(q4_2) : go(q4_4);
@@ -1081,7 +1080,7 @@ hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
 hipError_t launch_attn_merge(hipStream_t s, int nb, const AttnArgs &a) {
     const int64_t units = (int64_t)a.kv.n_seqs * a.row_tiles * a.kv.kv_heads;
     // a row a workgroup while the rows are few, else as many as fill it
-    const int rows = units * a.unit_rows <= 2048 ? 1 : kMergeThreads / (32 * nb);
+    const int rows = units * a.unit_rows <= 512 ? 1 : kMergeThreads / (32 * nb);
     const dim3 grid(units * (a.unit_rows / rows));
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kMergeThreads), 0, s, a, rows); };
     nb == 2 ? go(k_attn_merge<2>) : go(k_attn_merge<4>);

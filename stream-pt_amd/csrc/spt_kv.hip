@@ -21,7 +21,7 @@ namespace spt {
 
 namespace {
 
-constexpr int kStoreRows = 8;  // rows of a workgroup
+constexpr int kStoreRows = 4;  // rows of a workgroup
 
 // sin and cos of a >= 0 (or of either sign): n = a / (pi/2) rounded, r = a - n
 // pi/2 with pi/2 in two parts (each product exact in the FMA; n < 2^31), then
@@ -133,6 +133,7 @@ __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a, RopeTable rope)
     if (a.q) {
         const int h0 = (int)((int64_t)a.heads * part / a.parts), nh = (int)((int64_t)a.heads * (part + 1) / a.parts) - h0;
         constexpr int kQuads = kPairs / 4;
+#pragma unroll 4
         for (int u = tid; u < n * nh * kQuads; u += 256) {
             const int i = u % kQuads * 4, h = u / kQuads % nh, r = u / (kQuads * nh);
             const int64_t at = ((int64_t)(sq.r0 + i0 + r) * a.heads + h0 + h) * kDim + i;
@@ -223,10 +224,11 @@ __global__ __launch_bounds__(256) void k_kv_load(KvLoadArgs a) {
 }  // namespace
 
 // Few rows are shared by heads among up to kv_heads workgroups, while those
-// are fewer than two a compute unit.
+// are fewer than 16 a compute unit (4,099 rows of 64 query and 8 key/value heads
+// of 64: 40.3 us with two a compute unit and rows by eight, 31 us).
 int kv_store_parts(const KvArgs &a, int n_cu) {
     const int64_t chunks = (int64_t)((a.max_new + kStoreRows - 1) / kStoreRows) * a.n_seqs;
-    return (int)std::min<int64_t>(a.kv_heads, std::max<int64_t>(1, 2 * (int64_t)n_cu / chunks));
+    return (int)std::min<int64_t>(a.kv_heads, std::max<int64_t>(1, 16 * (int64_t)n_cu / chunks));
 }
 
 hipError_t launch_kv_store(hipStream_t s, int bits, int nb, const KvStoreArgs &a, const RopeTable &rope) {

@@ -230,6 +230,15 @@ def _numel(t):
     return int(t.size)
 
 
+def _f32(t):
+    """(elements, address) of an fp32 device tensor in C order; None: (0, None)."""
+    if t is None:
+        return 0, None
+    if t.element_size() != 4 or not t.is_contiguous():
+        raise ValueError("expected a contiguous fp32 tensor")
+    return t.numel(), t.data_ptr()
+
+
 def _check(rc):
     if rc != OK:
         raise SptError(rc, lib().spt_last_error().decode(errors="replace"))
@@ -381,14 +390,17 @@ class Context:
     def kv_store_batch(self, cache: KVCache, batch: KVBatch, k, v, rope: Rope = None, q=None, q_out=None):
         """Rotate the batch's queries (into q_out) and keys and write keys
         and values into the cache; rope None: keys as they are, no queries."""
-        nq = _numel(q) if q is not None else 0
-        no = _numel(q_out) if q_out is not None else 0
-        _check(lib().spt_kv_store_batch(self.handle, _ref(cache), _ref(batch), _ref(rope), _ptr(q), nq, _ptr(q_out), no,
-                                        _ptr(k), _numel(k), _ptr(v), _numel(v)))
+        nq, pq = _f32(q)
+        no, po = _f32(q_out)
+        nk, pk = _f32(k)
+        nv, pv = _f32(v)
+        _check(lib().spt_kv_store_batch(self.handle, _ref(cache), _ref(batch), _ref(rope), pq, nq, po, no, pk, nk, pv, nv))
 
     def kv_load_batch(self, cache: KVCache, batch: KVBatch, k, v):
         """The batch's rows of the cache as fp32 keys and values."""
-        _check(lib().spt_kv_load_batch(self.handle, _ref(cache), _ref(batch), _ptr(k), _numel(k), _ptr(v), _numel(v)))
+        nk, pk = _f32(k)
+        nv, pv = _f32(v)
+        _check(lib().spt_kv_load_batch(self.handle, _ref(cache), _ref(batch), pk, nk, pv, nv))
 
     def attention_work_bytes(self, cache: KVCache, batch: KVBatch, heads: int, window: int = 0) -> int:
         out = C.c_uint64()
@@ -400,9 +412,10 @@ class Context:
         """Attention of the batch's rows over the cache (forwardAttention);
         q8: GGML Q8_0 blocks of out; work: a uint8 buffer of
         attention_work_bytes, else the context's arena."""
-        _check(lib().spt_attention_batch_into(self.handle, _ref(cache), _ref(batch), _ref(sinks), scale, window, _ptr(q),
-                                              _numel(q), _ptr(out), _numel(out), _ptr(q8), _ptr(work),
-                                              _numel(work) if work is not None else 0))
+        nq, pq = _f32(q)
+        no, po = _f32(out)
+        _check(lib().spt_attention_batch_into(self.handle, _ref(cache), _ref(batch), _ref(sinks), scale, window, pq, nq, po, no,
+                                              _ptr(q8), _ptr(work), _numel(work) if work is not None else 0))
 
     def mul_mxfp4_expert(self, w: Tensor, bias, expert: int, x, y, batch: int):
         b = bias if bias is not None else Tensor.absent()
