@@ -114,7 +114,7 @@ typedef struct spt_moe_taps {
 
 /* A quantized key/value cache: n_pages pages of page_len positions, each
  * position n_kv_heads keys and values of head_dim elements in GGML blocks of
- * 32 (Q4_0: 18 bytes a block, 144 KB for 1,024 positions of 8 heads of 64;
+ * 32 (Q4_0: 18 bytes a block, 590 KB for 1,024 positions of 8 heads of 64;
  * Q8_0: 34).  The order of the bytes in a page is the library's own (a page
  * is copied whole); spt_kv_load_batch reads positions back.  head_dim is 64
  * or 128, page_len a multiple of 32.  Replaces forward.KVCache
@@ -145,7 +145,7 @@ typedef struct spt_kv_cache {
  * store may share a page that it writes, and no two rows a position. */
 typedef struct spt_kv_batch {
     int32_t n_seqs;    /* at most 65,535                                     */
-    int32_t max_new;   /* most rows of a sequence                            */
+    int32_t max_new;   /* most rows of a sequence (at most 2^24)             */
     int64_t n_rows;
     int64_t max_len;   /* longest sequence (at most 2^30 and max_pages * page_len) */
     int32_t max_pages; /* row length of pages_dev                            */

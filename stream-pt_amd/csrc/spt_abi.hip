@@ -1206,6 +1206,7 @@ int load_range(spt_ctx *ctx, const std::string &path, uint64_t start, uint64_t n
 int kv_type_bits(uint32_t type) { return type == SPT_TYPE_Q4_0 ? 4 : type == SPT_TYPE_Q8_0 ? 8 : 0; }
 
 constexpr int64_t kKvMaxLen = int64_t(1) << 30;  // positions of a sequence
+constexpr int32_t kKvMaxNew = 1 << 24;           // its rows in a call (a launch holds fewer than 2^32 threads)
 
 int kv_cache_size(uint32_t type, int64_t kv_heads, int64_t head_dim, int64_t page_len, int64_t n_pages, uint64_t *out) {
     if (!kv_type_bits(type))
@@ -1230,7 +1231,7 @@ int kv_check(const spt_kv_cache *c, const spt_kv_batch *b, int *bits, int *nb, s
     if (c->nbytes != bytes)
         return fail(SPT_ERR_INVALID, "key/value cache: %llu bytes instead of %llu", (unsigned long long)c->nbytes, (unsigned long long)bytes);
     if (!c->data || ((uintptr_t)c->data & 15)) return fail(SPT_ERR_INVALID, "key/value cache: data must be resident and 16-byte aligned");
-    if (b->n_seqs < 0 || b->n_seqs > 65535 || b->n_rows < 0 || b->n_rows > INT_MAX || b->max_new < 1 || b->max_len < 1 ||
+    if (b->n_seqs < 0 || b->n_seqs > 65535 || b->n_rows < 0 || b->n_rows > INT_MAX || b->max_new < 1 || b->max_new > kKvMaxNew || b->max_len < 1 ||
         b->max_len > kKvMaxLen || b->max_pages < 1)
         return fail(SPT_ERR_INVALID, "key/value batch: invalid sizes (%d sequences, %lld rows, at most %d new, %lld long, %d pages)", b->n_seqs,
                     (long long)b->n_rows, b->max_new, (long long)b->max_len, b->max_pages);

@@ -29,6 +29,7 @@
 // over 131,071, 28.4 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times that
 // with the halves): 110 us.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "spt_kernels.h"
@@ -127,10 +128,14 @@ __device__ inline void split_values(const Half8 &c, const u32x4 &d, Half8 &hi, H
     }
 }
 
-// The scales of eight positions, 0 from the one `left` on.
-__device__ inline void clear_scales(u32x4 &d, int left) {
+// The scales of eight positions, 0 outside [first, left): what is there belongs
+// to no row, and may be anything (a weight of 0 times NaN would be NaN).
+__device__ inline void clear_scales(u32x4 &d, int first, int left) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) d[i] = left <= 2 * i ? 0u : left == 2 * i + 1 ? d[i] & 0xFFFFu : d[i];
+    for (int i = 0; i < 4; i++) {
+        const uint32_t keep = (2 * i >= first && 2 * i < left ? 0xFFFFu : 0u) | (2 * i + 1 >= first && 2 * i + 1 < left ? 0xFFFF0000u : 0u);
+        d[i] &= keep;
+    }
 }
 __device__ inline u32x4 load16(rsrc_t tile, int lane_at, int at) {
     return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(tile, lane_at, at, 0));
@@ -192,11 +197,10 @@ struct RawTile {
             q8_codes(v[b][h * 2], v[b][h * 2 + 1], c);
         split_values(c, vs[b], hi, lo);
     }
-    // Positions from `left` on (of the lane's eight, at 8 g) are beyond the
-    // sequence: whatever is there counts as zero.
-    __device__ inline void clear_values(int left) {
+    // Only positions [first, left) of the lane's eight are any row's.
+    __device__ inline void clear_values(int first, int left) {
 #pragma unroll
-        for (int b = 0; b < NB; b++) clear_scales(vs[b], left);
+        for (int b = 0; b < NB; b++) clear_scales(vs[b], first, left);
     }
 };
 
@@ -209,10 +213,11 @@ constexpr int kMinWaves = NB == 2 ? 4 : 2;
 
 // A unit of work: a row tile (8, 16 or kManyRows rows) of a sequence and a
 // key/value head.  Its rows
-// are tokens [i_first, i_last]; the tiles [t_lo, t_hi) hold what they see.
+// are tokens [i_first, i_last]; the tiles [t_lo, t_hi) hold what they see, of
+// which p_lo is the first position.
 struct Unit {
     KvSeq sq;
-    int rows, i_first, i_last, t_lo, t_hi;
+    int rows, i_first, i_last, p_lo, t_lo, t_hi;
     __device__ inline int tiles() const { return max(1, t_hi - t_lo); }  // one that sees nothing is written too
 };
 
@@ -223,14 +228,14 @@ __device__ inline Unit unit_of(const AttnArgs &a, const KvSeq &sq, int rt) {
     u.sq = sq;
     u.rows = min(ROWS, u.sq.n * a.group - rt * ROWS);
     if (u.rows <= 0) {
-        u.rows = u.i_first = u.i_last = u.t_lo = u.t_hi = 0;
+        u.rows = u.i_first = u.i_last = u.p_lo = u.t_lo = u.t_hi = 0;
         return u;
     }
     u.i_first = rt * ROWS / a.group;
     u.i_last = (rt * ROWS + u.rows - 1) / a.group;
     const int last = u.sq.first + u.i_last;
-    const int lo = a.window ? max(0, u.sq.first + u.i_first - a.window + 1) : 0;
-    u.t_lo = lo / kKvTile;
+    u.p_lo = a.window ? max(0, u.sq.first + u.i_first - a.window + 1) : 0;
+    u.t_lo = u.p_lo / kKvTile;
     u.t_hi = last < 0 ? u.t_lo : last / kKvTile + 1;
     if (!u.sq.ok) u.t_lo = u.t_hi = 0;
     return u;
@@ -323,7 +328,7 @@ __device__ inline AttnWork attn_work(const AttnArgs &a) {
     const int64_t units = (int64_t)a.kv.n_seqs * a.row_tiles * a.kv.kv_heads;
     AttnWork w;
     w.units = reinterpret_cast<int2 *>(a.work);
-    w.tops = reinterpret_cast<float2 *>(w.units + units);
+    w.tops = reinterpret_cast<float2 *>(w.units + (units + 1) / 2 * 2);  // outputs are stored by 16 bytes
     w.outs = reinterpret_cast<float *>(w.tops + (a.groups + units) * a.unit_rows);
     return w;
 }
@@ -492,7 +497,7 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
                 const int p = mine + j;
                 x[j] = p <= pos && p > from ? x[j] : -__builtin_inff();
             }
-            if (p0 + kKvTile > sq.len) raw.clear_values(sq.len - p0 - 8 * g);
+            if (p0 < un.p_lo || p0 + kKvTile > sq.len) raw.clear_values(un.p_lo - p0 - 8 * g, sq.len - p0 - 8 * g);
         }
 #pragma unroll
         for (int j = 0; j < kMine; j++) top = fmaxf(top, x[j]);
@@ -661,8 +666,8 @@ struct ManyPart {
             }
         }
     }
-    // left: positions of the tile before the sequence's end.
-    __device__ inline void make(const Opaque &o, typename ManyLds<NB>::Buffer &buf, int left, int wave, int lane) {
+    // Positions [first, left) of the tile are some row's.
+    __device__ inline void make(const Opaque &o, typename ManyLds<NB>::Buffer &buf, int first, int left, int wave, int lane) {
 #pragma unroll
         for (int j = 0; j < kUnits; j++) {
             const int u = wave % kHalf * kUnits + j;
@@ -683,7 +688,7 @@ struct ManyPart {
                 } else {
                     q8_codes(c[j].x, c[j].y, v);
                 }
-                if (left < kKvTile) clear_scales(d[j], left - 8 * (lane >> 4));
+                if (first > 0 || left < kKvTile) clear_scales(d[j], first - 8 * (lane >> 4), left - 8 * (lane >> 4));
                 split_values(v, d[j], hi, lo);
                 buf.v[u][0][lane] = hi;
                 buf.v[u][1][lane] = lo;
@@ -819,11 +824,11 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
             }
     };
 
-    raw.make(oc, lds.buf[0], sq.len - t_begin * kKvTile, wave, lane);
+    raw.make(oc, lds.buf[0], un.p_lo - t_begin * kKvTile, sq.len - t_begin * kKvTile, wave, lane);
     load();
     lds_barrier();
     auto step = [&](int t, int now) __attribute__((always_inline)) {
-        raw.make(oc, lds.buf[now ^ 1], sq.len - (t + 1) * kKvTile, wave, lane);
+        raw.make(oc, lds.buf[now ^ 1], un.p_lo - (t + 1) * kKvTile, sq.len - (t + 1) * kKvTile, wave, lane);
         load();
         take(lds.buf[now], t);
         lds_barrier();
@@ -1050,10 +1055,11 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
     const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
     const int64_t resident = (int64_t)n_cu * 4 * (many || nb == 4 ? 2 : kMinWaves<2>) / kWaves;  // workgroups at once
     const bool direct = many ? units >= resident : rows > kFewRows || tiles <= std::max<int64_t>(kDirectTiles, std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu));
-    if (!direct && entries <= kAttnEntries) {
-        const int64_t cost = many ? kManyCost : kUnitCost;
+    const int64_t cost = many ? kManyCost : kUnitCost;
+    // (the shares' sums are 32 bits, their merge a workgroup a unit at least)
+    if (!direct && entries <= kAttnEntries && units <= (1 << 18) && entries * (tiles + cost) <= INT_MAX) {
         p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + cost) / cost));
-        p.work_bytes = (uint64_t)units * 8 + (uint64_t)(units + p.groups) * p.unit_rows * (8 + 128 * nb);
+        p.work_bytes = (uint64_t)(units + 1) / 2 * 16 + (uint64_t)(units + p.groups) * p.unit_rows * (8 + 128 * nb);
     }
     return p;
 }

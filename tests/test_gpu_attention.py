@@ -117,6 +117,71 @@ def test_long_sequences(gpu_ctx, bits, dim, kv, group, new, lens, window):
         assert np.array_equal(got, run(gpu_ctx, p, q, dim ** -0.5, window, sk, work=work))
 
 
+# Row tiles of 256 rows, paired: so many heads that the row tiles are more than the compute units.
+PAIRS = [
+    (4, 64, 64, 4, [70, 66], [70, 300], 0, True),
+    (8, 64, 130, 4, [130, 0], [130, 9], 37, False),
+    (4, 128, 64, 3, [86, 171], [90, 171], 0, False),
+    (8, 128, 32, 16, [49, 50, 17, 1], [49, 177, 17, 260], 20, True),
+]
+
+
+@pytest.mark.parametrize("bits,dim,kv,group,new,lens,window,sinks", PAIRS)
+def test_paired_row_tiles(gpu_ctx, bits, dim, kv, group, new, lens, window, sinks):
+    p = Filled(gpu_ctx, bits, kv, dim, 32, new, lens, seed=kv, peak=12.0 / np.sqrt(dim), extra_rows=1)
+    q = p.rng.standard_normal((p.n_rows, kv * group, dim)).astype(np.float32)
+    sk = (p.rng.standard_normal(kv * group) * 2).astype(np.float32) if sinks else None
+    got, blocks = run(gpu_ctx, p, q, dim ** -0.5, window, sk, q8=True)
+    check(got, *p.want(q, dim ** -0.5, window, sk))
+    assert (got[-1] == 9.0).all()
+    import torch
+
+    n = sum(new) * kv * group * dim
+    blk = torch.empty(n // 32 * 34, dtype=torch.uint8, device="cuda")
+    gpu_ctx.quantize_q8_0(_cuda(got[:sum(new)]), blk)
+    assert torch.equal(blocks[:blk.numel()], blk) and bool((blocks[blk.numel():] == 0xAA).all())
+
+
+def test_paired_row_tiles_that_cannot_see(gpu_ctx):
+    """Marked keys, pages that are none and rows before the first position, 256 rows at a time."""
+    kv, new = 130, 67
+    p = Filled(gpu_ctx, 4, kv, 64, 32, [new, new], [100, 40])
+    b, starts, n = p.whole()
+    k, v = (p.rng.standard_normal((n, kv, 64)).astype(np.float32) for _ in range(2))
+    k[50, 3, 1] = np.nan
+    gpu_ctx.kv_store_batch(p.cache, b, _cuda(k), _cuda(v))
+    ks, vs = stored(k, v, 4)
+    p.k, p.v = [ks[:100], ks[100:]], [vs[:100], vs[100:]]
+    q = p.rng.standard_normal((2 * new, kv * 4, 64)).astype(np.float32)
+    table = p.table.copy()
+    table[0, 2] = -1  # positions 64 .. 95
+    got = run(gpu_ctx, p, q, 0.125, batch=p.make_batch(p.starts, p.lens, new, 100, table=table))
+    pos = np.arange(100 - new, 100)
+    bad = np.repeat((pos >= 64)[:, None], kv * 4, 1)
+    bad[pos >= 50, 12:16] = True
+    assert np.array_equal(np.isnan(got[:new]).all(-1), bad) and np.array_equal(np.isnan(got[:new]).any(-1), bad)
+    want, tol = p.want(q, 0.125)
+    assert (np.abs(got[:new] - want[:new])[~bad] <= tol[:new][~bad]).all()
+    assert (got[new:2 * new - 40] == 0).all()
+    assert (np.abs(got[new:] - want[new:]) <= tol[new:]).all()
+
+
+@pytest.mark.parametrize("bits,kv,new,window,length", [(4, 1, 1, 20, 90), (8, 1, 4, 20, 90), (4, 1, 40, 9, 90), (4, 130, 67, 5, 100), (8, 2, 40, 100, 4000)])
+def test_only_the_window_was_stored(gpu_ctx, bits, kv, new, window, length):
+    """Positions that no row sees hold anything (scales of NaN), in the same
+    tiles as those that rows see: before the window and behind the end."""
+    p = Paged(bits, kv, 64, 64, [new], [length], seed=2)
+    p.data.fill_(0xFF)
+    n = min(length, new + window - 1)
+    k, v = (p.rng.standard_normal((n, kv, 64)).astype(np.float32) for _ in range(2))
+    gpu_ctx.kv_store_batch(p.cache, p.make_batch([0, n], [length], n, length, n_rows=n), _cuda(k), _cuda(v))
+    ks, vs = stored(k, v, bits)
+    full = np.zeros((length, kv, 64), np.float32), np.zeros((length, kv, 64), np.float32)
+    full[0][length - n:], full[1][length - n:] = ks, vs
+    q = p.rng.standard_normal((new, kv * 4, 64)).astype(np.float32)
+    check(run(gpu_ctx, p, q, 0.125, window), *attend(q, *full, length - new, 0.125, window))
+
+
 def test_rows_of_a_batch_are_independent(gpu_ctx):
     """A sequence's rows have the same bits alone and beside others."""
     p = Filled(gpu_ctx, 4, 2, 64, 32, [3, 50, 1], [40, 50, 333], seed=8)

@@ -85,6 +85,7 @@ COMMON = {
     "many rows": lambda c: setattr(c.batch, "n_rows", 1 << 40),
     "rows of the buffers": lambda c: setattr(c.batch, "n_rows", 8),
     "no new": lambda c: setattr(c.batch, "max_new", 0),
+    "many new": lambda c: setattr(c.batch, "max_new", (1 << 24) + 1),
     "no length": lambda c: setattr(c.batch, "max_len", 0),
     "long": lambda c: (setattr(c.batch, "max_len", (1 << 30) + 1), setattr(c.batch, "max_pages", 1 << 29)),
     "no page table": lambda c: setattr(c.batch, "max_pages", 0),
