@@ -17,7 +17,7 @@
 // each or two): the workgroup's waves take tiles of 32 positions in turn and
 // make their operands in registers; a tile's scores are its D registers, and
 // those are the B operand of the product with the values.  Many rows
-// (attend_many: 256 at a time): operands are made once a workgroup in LDS.  The
+// (attend_many: 128 at a time): operands are made once a workgroup in LDS.  The
 // running maximum is one number a row, raised only when a score passes it by
 // kSlack (weights up to 2^kSlack fit fp16 beside the lift), so most tiles need
 // no exchange between lanes and no rescaling.
@@ -45,19 +45,19 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 8;  // of a workgroup (few rows)
-// Launches, by what the batch's bounds allow (us, one token of 64 heads on 8 of 64
-// unless said otherwise):
-//   rows of a key/value head: up to 8, two columns a row (an 8-head token, 64 ragged
-//   sequences up to 8,192: 59, a column a row 70); up to kFewRows, 16 at a
-//   time; more, 256 at a time, except where 16 at a time are at most a workgroup a
-//   compute unit and kChunkTiles tiles long (32 tokens over 2,049 positions: 13, 256
-//   at a time 33);
-//   a workgroup a unit (a row tile of a sequence and head) up to kDirectTiles position
-//   tiles, and further, up to kWideTiles, in proportion to the units while they do
-//   not fill the compute units (1 sequence of 2,048: 11.5, shares 12.8; of 4,096:
-//   18.3, 13.2; 64 ragged ones up to 4,096: 31, 40; up to 16,384: 104, 97); beyond,
-//   equal shares of all tiles and a second launch.
-constexpr int kFewRows = 32, kChunkTiles = 96, kDirectTiles = 72, kWideTiles = 300;
+// Launches, by what the batch's bounds allow (us; heads 64 on 8 of 64, Q4_0):
+//   rows of a key/value head: up to 8, two columns a row (a token of 64 ragged
+//   sequences up to 8,192: 59, a column a row 70); up to kFewRows, 16 at a time (64
+//   tokens over 16,000 positions: 74, 128 at a time 78; of 8 ragged sequences
+//   up to 4,000: 75, 103; 128 tokens of 32 up to 2,000: 265, 220); more, 128 at a time,
+//   except where 16 at a time are at most a workgroup a compute unit and kChunkTiles
+//   tiles long.
+//   Few rows: a workgroup a unit (a row tile of a sequence and head) up to kDirectTiles
+//   position tiles, and further, up to kWideTiles, in proportion to the units while they
+//   do not fill the compute units (a token of 1 sequence of 2,048: 11.5, shares
+//   12.8; of 4,096: 18.3, 13.2; of 64 ragged ones up to 4,096: 31, 40; up to 16,384:
+//   104, 97); beyond, equal shares of all tiles and a second launch.
+constexpr int kFewRows = 512, kChunkTiles = 96, kDirectTiles = 72, kWideTiles = 300;
 constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup of the shares sums up
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
@@ -615,14 +615,13 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_units(AttnA
     if (u.rows) attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
 }
 
-// Rows many at a time: a workgroup's 8 waves have 32 rows each (two columns of
+// Rows many at a time: a workgroup's 4 waves have 32 rows each (two columns of
 // the MFMA), and share the tiles' operands, made once a workgroup in LDS: key
 // codes, and values as hi and lo.  While one tile is taken from one buffer, the
 // next is made in the other and the bytes of the one after it are on their
-// way.  Each wave makes an eighth of a tile: a unit is a key or value operand of
+// way.  Each wave makes a quarter of a tile: a unit is a key or value operand of
 // one MFMA, 1 KB or twice 1 KB.
-constexpr int kManyWaves = 8, kManyRows = 32 * kManyWaves;
-static_assert(kManyWaves == kWaves, "one launch shape");
+constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 
 template <int NB>
 union ManyLds {
@@ -875,20 +874,17 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
     }
 }
 
-// A workgroup a pair of units, the last row tile with the first, and so on
-// inward: the causal ones then have about the same number of tiles.
+// A workgroup a unit, the last row tiles first: the causal ones with the most
+// tiles, so that the short ones even out the end.
 template <int BITS, int NB>
-__global__ __launch_bounds__(64 * kManyWaves, 2) void k_attn_pairs(AttnArgs a) {
+__global__ __launch_bounds__(64 * kManyWaves, 2) void k_attn_many(AttnArgs a) {
     __shared__ ManyLds<NB> lds;
-    const int kvh = blockIdx.x % a.kv.kv_heads, pair = blockIdx.x / a.kv.kv_heads, seq = blockIdx.y;
+    const int kvh = blockIdx.x % a.kv.kv_heads, seq = blockIdx.y;
     const KvSeq sq = kv_seq(a.kv, seq);
-    const int tiles = (sq.n * a.group + kManyRows - 1) / kManyRows;
-    for (int i = 0; i < 2; i++) {
-        const int rt = i ? pair : tiles - 1 - pair;
-        if (i ? pair >= tiles - 1 - pair : rt < pair) return;
-        const Unit u = unit_of<kManyRows>(a, sq, rt);
-        attend_many<BITS, NB>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
-    }
+    const int rt = (sq.n * a.group + kManyRows - 1) / kManyRows - 1 - (int)(blockIdx.x / a.kv.kv_heads);
+    if (rt < 0) return;
+    const Unit u = unit_of<kManyRows>(a, sq, rt);
+    attend_many<BITS, NB>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
 }
 
 // All units' tiles in a row, cut into equal shares, one a workgroup: however
@@ -899,13 +895,13 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void k_attn_pairs(AttnArgs a) {
 // workgroup or a new unit.
 constexpr int kUnitCost = 16, kManyCost = 2;
 template <int BITS, int NB, int ROWS>
-__global__ __launch_bounds__(64 * kWaves, ROWS == kManyRows ? 2 : kMinWaves<NB>) void k_attn_shares(AttnArgs a) {
+__global__ __launch_bounds__(64 * (ROWS == kManyRows ? kManyWaves : kWaves), ROWS == kManyRows ? 2 : kMinWaves<NB>) void k_attn_shares(AttnArgs a) {
     constexpr bool MANY = ROWS == kManyRows;
     constexpr int kCost = MANY ? kManyCost : kUnitCost;
-    constexpr int kThreads = 64 * kWaves, kEach = kAttnEntries / kThreads;
+    constexpr int kGroupWaves = MANY ? kManyWaves : kWaves, kThreads = 64 * kGroupWaves, kEach = kAttnEntries / kThreads;
     __shared__ std::conditional_t<MANY, ManyLds<NB>, AttnLds<NB>> lds;
     __shared__ int before[kAttnEntries + 1];  // cost of a head before each (sequence, row tile)
-    __shared__ int wave_sum[kWaves];
+    __shared__ int wave_sum[kGroupWaves];
     const int entries = a.kv.n_seqs * a.row_tiles, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int n[kEach], sum = 0;
 #pragma unroll
@@ -929,7 +925,7 @@ __global__ __launch_bounds__(64 * kWaves, ROWS == kManyRows ? 2 : kMinWaves<NB>)
     __syncthreads();
     int at = scan - sum, total = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
+    for (int w = 0; w < kGroupWaves; w++) {
         if (w < wave) at += wave_sum[w];
         total += wave_sum[w];
     }
@@ -1053,8 +1049,11 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
     const bool many = p.unit_rows == kManyRows;
     p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
     const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
-    const int64_t resident = (int64_t)n_cu * 4 * (many || nb == 4 ? 2 : kMinWaves<2>) / kWaves;  // workgroups at once
-    const bool direct = many ? units >= resident : rows > kFewRows || tiles <= std::max<int64_t>(kDirectTiles, std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu));
+    // workgroups at once
+    const int64_t resident = (int64_t)n_cu * 4 * (many || nb == 4 ? 2 : kMinWaves<2>) / (many ? kManyWaves : kWaves);
+    // 128 rows at a time, us: 1.25 a tile one workgroup a unit, about 18 and 2 a tile of a
+    // workgroup's share in shares (768 tokens 39, 65; 128 over 8,192: 320, 80)
+    const bool direct = many ? 5 * tiles * resident <= 72 * resident + 8 * units * tiles : rows > kFewRows || tiles <= std::max<int64_t>(kDirectTiles, std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu));
     const int64_t cost = many ? kManyCost : kUnitCost;
     // (the shares' sums are 32 bits, their merge a workgroup a unit at least)
     if (!direct && entries <= kAttnEntries && units <= (1 << 18) && entries * (tiles + cost) <= INT_MAX) {
@@ -1066,8 +1065,8 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
 
 hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
     const bool many = a.unit_rows == kManyRows;
-    const dim3 grid = a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * (many ? (a.row_tiles + 1) / 2 : a.row_tiles), a.kv.n_seqs);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * kWaves), 0, s, a); };
+    const dim3 grid = a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * a.row_tiles, a.kv.n_seqs);
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, a); };
     auto pick = [&](auto q4_2, auto q4_4, auto q8_2, auto q8_4) {
         if (bits == 4)
             nb == 2 ? go(q4_2) : go(q4_4);
@@ -1078,7 +1077,7 @@ hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
     if (a.groups)
         many ? SPT_PICK(k_attn_shares, kManyRows) : a.unit_rows == 8 ? SPT_PICK(k_attn_shares, 8) : SPT_PICK(k_attn_shares, 16);
     else
-        many ? SPT_PICK(k_attn_pairs) : a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8) : SPT_PICK(k_attn_units, 16);
+        many ? SPT_PICK(k_attn_many) : a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8) : SPT_PICK(k_attn_units, 16);
 #undef SPT_PICK
     return hipGetLastError();
 }

@@ -117,17 +117,21 @@ def test_long_sequences(gpu_ctx, bits, dim, kv, group, new, lens, window):
         assert np.array_equal(got, run(gpu_ctx, p, q, dim ** -0.5, window, sk, work=work))
 
 
-# Row tiles of 256 rows, paired: so many heads that the row tiles are more than the compute units.
-PAIRS = [
-    (4, 64, 64, 4, [70, 66], [70, 300], 0, True),
+# Many rows a head, 128 at a time: a workgroup a row tile where there are many, shares of few long ones.
+MANY = [
+    (4, 64, 64, 4, [140, 133], [140, 300], 0, True),
     (8, 64, 130, 4, [130, 0], [130, 9], 37, False),
     (4, 128, 64, 3, [86, 171], [90, 171], 0, False),
     (8, 128, 32, 16, [49, 50, 17, 1], [49, 177, 17, 260], 20, True),
+    (8, 128, 16, 16, [65], [65], 0, True),
+    (4, 64, 1, 17, [31, 40], [3333, 40], 0, True),
+    (8, 128, 1, 8, [65], [4000], 0, False),
+    (8, 64, 1, 8, [65, 1], [4000, 5000], 3500, True),
 ]
 
 
-@pytest.mark.parametrize("bits,dim,kv,group,new,lens,window,sinks", PAIRS)
-def test_paired_row_tiles(gpu_ctx, bits, dim, kv, group, new, lens, window, sinks):
+@pytest.mark.parametrize("bits,dim,kv,group,new,lens,window,sinks", MANY)
+def test_many_rows(gpu_ctx, bits, dim, kv, group, new, lens, window, sinks):
     p = Filled(gpu_ctx, bits, kv, dim, 32, new, lens, seed=kv, peak=12.0 / np.sqrt(dim), extra_rows=1)
     q = p.rng.standard_normal((p.n_rows, kv * group, dim)).astype(np.float32)
     sk = (p.rng.standard_normal(kv * group) * 2).astype(np.float32) if sinks else None
@@ -142,8 +146,8 @@ def test_paired_row_tiles(gpu_ctx, bits, dim, kv, group, new, lens, window, sink
     assert torch.equal(blocks[:blk.numel()], blk) and bool((blocks[blk.numel():] == 0xAA).all())
 
 
-def test_paired_row_tiles_that_cannot_see(gpu_ctx):
-    """Marked keys, pages that are none and rows before the first position, 256 rows at a time."""
+def test_many_rows_that_cannot_see(gpu_ctx):
+    """Marked keys, pages that are none and rows before the first position, 128 rows at a time."""
     kv, new = 130, 67
     p = Filled(gpu_ctx, 4, kv, 64, 32, [new, new], [100, 40])
     b, starts, n = p.whole()
@@ -152,13 +156,13 @@ def test_paired_row_tiles_that_cannot_see(gpu_ctx):
     gpu_ctx.kv_store_batch(p.cache, b, _cuda(k), _cuda(v))
     ks, vs = stored(k, v, 4)
     p.k, p.v = [ks[:100], ks[100:]], [vs[:100], vs[100:]]
-    q = p.rng.standard_normal((2 * new, kv * 4, 64)).astype(np.float32)
+    q = p.rng.standard_normal((2 * new, kv * 8, 64)).astype(np.float32)
     table = p.table.copy()
     table[0, 2] = -1  # positions 64 .. 95
     got = run(gpu_ctx, p, q, 0.125, batch=p.make_batch(p.starts, p.lens, new, 100, table=table))
     pos = np.arange(100 - new, 100)
-    bad = np.repeat((pos >= 64)[:, None], kv * 4, 1)
-    bad[pos >= 50, 12:16] = True
+    bad = np.repeat((pos >= 64)[:, None], kv * 8, 1)
+    bad[pos >= 50, 24:32] = True
     assert np.array_equal(np.isnan(got[:new]).all(-1), bad) and np.array_equal(np.isnan(got[:new]).any(-1), bad)
     want, tol = p.want(q, 0.125)
     assert (np.abs(got[:new] - want[:new])[~bad] <= tol[:new][~bad]).all()
@@ -166,7 +170,7 @@ def test_paired_row_tiles_that_cannot_see(gpu_ctx):
     assert (np.abs(got[new:] - want[new:]) <= tol[new:]).all()
 
 
-@pytest.mark.parametrize("bits,kv,new,window,length", [(4, 1, 1, 20, 90), (8, 1, 4, 20, 90), (4, 1, 40, 9, 90), (4, 130, 67, 5, 100), (8, 2, 40, 100, 4000)])
+@pytest.mark.parametrize("bits,kv,new,window,length", [(4, 1, 1, 20, 90), (8, 1, 4, 20, 90), (4, 1, 40, 9, 90), (4, 130, 129, 5, 200), (8, 2, 129, 3100, 4000)])
 def test_only_the_window_was_stored(gpu_ctx, bits, kv, new, window, length):
     """Positions that no row sees hold anything (scales of NaN), in the same
     tiles as those that rows see: before the window and behind the end."""
