@@ -497,7 +497,7 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
                 const int p = mine + j;
                 x[j] = p <= pos && p > from ? x[j] : -__builtin_inff();
             }
-            if (p0 < un.p_lo || p0 + kKvTile > sq.len) raw.clear_values(un.p_lo - p0 - 8 * g, sq.len - p0 - 8 * g);
+            raw.clear_values(un.p_lo - p0 - 8 * g, sq.len - p0 - 8 * g);
         }
 #pragma unroll
         for (int j = 0; j < kMine; j++) top = fmaxf(top, x[j]);
@@ -687,7 +687,10 @@ struct ManyPart {
                 } else {
                     q8_codes(c[j].x, c[j].y, v);
                 }
-                if (first > 0 || left < kKvTile) clear_scales(d[j], first - 8 * (lane >> 4), left - 8 * (lane >> 4));
+                if (first > 0 || left < kKvTile) {
+                    asm volatile("");  // a branch: few tiles are an end
+                    clear_scales(d[j], first - 8 * (lane >> 4), left - 8 * (lane >> 4));
+                }
                 split_values(v, d[j], hi, lo);
                 buf.v[u][0][lane] = hi;
                 buf.v[u][1][lane] = lo;
@@ -996,8 +999,8 @@ __global__ __launch_bounds__(kMergeThreads) void k_attn_merge(AttnArgs a, int ro
     const int e = (int)(unit / a.kv.kv_heads), kvh = (int)(unit % a.kv.kv_heads), seq = e / a.row_tiles, rt = e % a.row_tiles;
     const KvSeq sq = kv_seq(a.kv, seq);
     const int n_rows = min(a.unit_rows, sq.n * a.group - rt * a.unit_rows);
+    const int2 wg = w.units[unit];  // (read beside the sequence; of no unit where it has no rows)
     if (chunk * rows >= n_rows) return;
-    const int2 wg = w.units[unit];
     const int n = wg.y - wg.x + 1;
     if (n <= 1) return;
     const int tid = threadIdx.x, lane = tid & 63, d = tid % kDim, groups = kMergeThreads / kDim / rows;
