@@ -26,8 +26,8 @@
 // and the MFMAs, which overlap with them in part only (16 MFMAs and 64 FMAs of
 // two waves on a SIMD, one wave each: 463 cycles, 319 and 322 alone).  One
 // token over 1,048,576 positions of 8 heads of 64 (604 MB) takes 144 us, 4.2 TB/s;
-// over 131,071, 28.4 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times that
-// with the halves): 110 us.
+// over 131,071, 28 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times that
+// with the halves): 110 us; of 8,192, 1.31 ms (1,040 TFLOP/s of MFMA).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
