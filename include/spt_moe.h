@@ -142,7 +142,9 @@ typedef struct spt_kv_cache {
  * max_new rows or longer than max_len is not stored, and its first max_new
  * rows load and attend as NaN (its others are left as they were).  Rows
  * that belong to no sequence are left as they were.  No two sequences of a
- * store may share a page that it writes, and no two rows a position. */
+ * store may share a page that it writes, and no two rows a position; rows that
+ * two sequences claim (a rows_dev that falls) hold the results of either.
+ * What a call writes may not overlap these arrays. */
 typedef struct spt_kv_batch {
     int32_t n_seqs;    /* at most 65,535                                     */
     int32_t max_new;   /* most rows of a sequence (at most 2^24)             */

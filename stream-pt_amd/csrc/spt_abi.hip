@@ -1223,6 +1223,13 @@ int kv_cache_size(uint32_t type, int64_t kv_heads, int64_t head_dim, int64_t pag
     return SPT_OK;
 }
 
+// Whether memory that a call writes is the batch's arrays, which its kernels read as constants.
+bool overlaps_batch(const void *p, uint64_t n, const spt_kv_batch *b) {
+    const uint64_t seqs = (uint64_t)b->n_seqs;
+    return ranges_overlap(p, n, b->rows_dev, (seqs + 1) * 4) || ranges_overlap(p, n, b->lens_dev, seqs * 4) ||
+           ranges_overlap(p, n, b->pages_dev, seqs * (uint64_t)b->max_pages * 4);
+}
+
 int kv_check(const spt_kv_cache *c, const spt_kv_batch *b, int *bits, int *nb, spt::KvArgs *a) {
     if (!c || !b) return fail(SPT_ERR_INVALID, "nil key/value cache or batch");
     uint64_t bytes;
@@ -1239,6 +1246,7 @@ int kv_check(const spt_kv_cache *c, const spt_kv_batch *b, int *bits, int *nb, s
         return fail(SPT_ERR_INVALID, "key/value batch: %lld positions do not fit %d pages of %d", (long long)b->max_len, b->max_pages, c->page_len);
     if (!b->rows_dev || !b->lens_dev || !b->pages_dev || (((uintptr_t)b->rows_dev | (uintptr_t)b->lens_dev | (uintptr_t)b->pages_dev) & 3))
         return fail(SPT_ERR_INVALID, "key/value batch: nil or unaligned rows, lengths or pages");
+    if (overlaps_batch(c->data, c->nbytes, b)) return fail(SPT_ERR_INVALID, "the key/value cache overlaps the batch's rows, lengths or pages");
     if (bytes / (uint64_t)c->n_pages > 0x7FFFFFFFull)
         return fail(SPT_ERR_INVALID, "key/value cache: a page of %llu bytes is too large", (unsigned long long)(bytes / (uint64_t)c->n_pages));
     *bits = kv_type_bits(c->type);
@@ -1257,6 +1265,7 @@ int kv_rows_check(const char *what, const float *p, int64_t len, int64_t heads, 
                     (long long)heads, c->head_dim);
     if (len && (!p || ((uintptr_t)p & 15))) return fail(SPT_ERR_INVALID, "%s: nil or not 16-byte aligned", what);
     if (ranges_overlap(p, (uint64_t)len * 4, c->data, c->nbytes)) return fail(SPT_ERR_INVALID, "%s overlaps the key/value cache", what);
+    if (overlaps_batch(p, (uint64_t)len * 4, b)) return fail(SPT_ERR_INVALID, "%s overlaps the batch's rows, lengths or pages", what);
     return SPT_OK;
 }
 
@@ -1866,14 +1875,18 @@ int spt_attention_batch_into(spt_ctx *ctx, const spt_kv_cache *cache, const spt_
     if (!elements_aligned(sk)) return fail(SPT_ERR_INVALID, "\"%s\": data must be aligned to its elements", tname(&sk));
     const uint64_t qb = (uint64_t)q_len * 4, q8b = q8_dev ? (uint64_t)q_len / 32 * 34 : 0;
     if (ranges_overlap(q_dev, qb, out_dev, qb)) return fail(SPT_ERR_INVALID, "attention: queries and output overlap");
-    if (ranges_overlap(q8_dev, q8b, q_dev, qb) || ranges_overlap(q8_dev, q8b, out_dev, qb) || ranges_overlap(q8_dev, q8b, cache->data, cache->nbytes))
-        return fail(SPT_ERR_INVALID, "attention: Q8_0 output overlaps the queries, the output or the cache");
+    const uint64_t sb = bias_bytes(sk);
+    if (ranges_overlap(out_dev, qb, sk.data, sb)) return fail(SPT_ERR_INVALID, "attention: output overlaps the sinks");
+    if (ranges_overlap(q8_dev, q8b, q_dev, qb) || ranges_overlap(q8_dev, q8b, out_dev, qb) || ranges_overlap(q8_dev, q8b, cache->data, cache->nbytes) ||
+        ranges_overlap(q8_dev, q8b, sk.data, sb) || overlaps_batch(q8_dev, q8b, batch))
+        return fail(SPT_ERR_INVALID, "attention: Q8_0 output overlaps an input or the output");
     if (work_dev) {
         if (((uintptr_t)work_dev & 15) || work_bytes < call.work_bytes)
             return fail(SPT_ERR_INVALID, "attention: the workspace must be 16-byte aligned and hold %llu bytes, got %llu",
                         (unsigned long long)call.work_bytes, (unsigned long long)work_bytes);
         if (ranges_overlap(work_dev, call.work_bytes, q_dev, qb) || ranges_overlap(work_dev, call.work_bytes, out_dev, qb) ||
-            ranges_overlap(work_dev, call.work_bytes, q8_dev, q8b) || ranges_overlap(work_dev, call.work_bytes, cache->data, cache->nbytes))
+            ranges_overlap(work_dev, call.work_bytes, q8_dev, q8b) || ranges_overlap(work_dev, call.work_bytes, cache->data, cache->nbytes) ||
+            ranges_overlap(work_dev, call.work_bytes, sk.data, sb) || overlaps_batch(work_dev, call.work_bytes, batch))
             return fail(SPT_ERR_INVALID, "attention: the workspace overlaps an input or output");
     }
     if ((rc = check_device(ctx)) || (rc = check_cancel(ctx))) return rc;

@@ -110,7 +110,7 @@ __device__ inline void store_blocks(uint8_t *tile, int p, const float (&x)[NB / 
     }
 }
 
-// Rows [8 x, 8 x + 8) of sequence y, heads of part z: angles of the rows into
+// Rows [4 x, 4 x + 4) of sequence y, heads of part z: angles of the rows into
 // LDS, then query pairs by threads and keys and values by waves.
 template <int BITS, int NB>
 __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a, RopeTable rope) {

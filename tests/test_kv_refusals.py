@@ -225,3 +225,36 @@ def test_python_descriptors_check_their_tensors():
     for bad in ((rows.long(), lens, pages), (rows, lens, pages.T.contiguous()), (rows, lens, pages[:, ::2]), (rows[:2], lens, pages)):
         with pytest.raises(ValueError):
             spt.KVBatch.make(*bad, 1, 1, 1)
+
+
+@pytest.mark.parametrize("array", ("rows_dev", "lens_dev", "pages_dev"))
+@pytest.mark.parametrize("entry,what", [("store", "out"), ("store", "cache"), ("load", "k"), ("load", "v"), ("load", "cache"),
+                                        ("attend", "out"), ("attend", "q8"), ("attend", "work"), ("attend", "cache")])
+def test_the_batch_is_not_written(ctx, entry, what, array):
+    """What a call writes may not be the batch's arrays, which it reads."""
+    import spt
+
+    c = Call()
+    if what == "work":
+        c.cache = spt.KVCache.make(spt.TYPE_Q4_0, 2, 64, 64, 5, 1 << 44)
+        c.batch.max_pages, c.batch.max_len = 4096, 200000
+        c.work, c.work_bytes = 0x40000000, ctx.attention_work_bytes(c.cache, c.batch, 6)
+        c.batch.rows_dev, c.batch.lens_dev, c.batch.pages_dev = 0x3000000, 0x4000000, 0x5000000
+    assert getattr(c, entry)(ctx) == spt.ERR_DEVICE
+    c.q8 = 0x30000000 if what == "q8" else None
+    setattr(c.batch, array, (c.cache.data if what == "cache" else getattr(c, what)) + 32)
+    assert getattr(c, entry)(ctx) == spt.ERR_INVALID
+
+
+@pytest.mark.parametrize("what", ("out", "q8", "work"))
+def test_sinks_are_not_written(ctx, what):
+    import spt
+
+    c = Call()
+    c.cache = spt.KVCache.make(spt.TYPE_Q4_0, 2, 64, 64, 5, 1 << 44)
+    c.batch.max_pages, c.batch.max_len = 4096, 200000
+    c.work, c.work_bytes, c.q8 = 0x40000000, ctx.attention_work_bytes(c.cache, c.batch, 6), 0x30000000
+    _sinks(c)
+    assert c.attend(ctx) == spt.ERR_DEVICE
+    c.sinks.data = getattr(c, what) + 32
+    assert c.attend(ctx) == spt.ERR_INVALID
