@@ -1868,7 +1868,7 @@ int spt_attention_batch_into(spt_ctx *ctx, const spt_kv_cache *cache, const spt_
     if (out_len != q_len) return fail(SPT_ERR_INVALID, "attention: %lld elements of queries and %lld of output", (long long)q_len, (long long)out_len);
     if ((rc = kv_rows_check("queries", q_dev, q_len, heads, cache, batch))) return rc;
     if ((rc = kv_rows_check("attention output", out_dev, out_len, heads, cache, batch))) return rc;
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(SPT_ERR_INVALID, "attention: invalid scale %g", (double)scale);
+    if (!(scale > 0.0f) || !std::isfinite(scale * 1.44269504088896341f)) return fail(SPT_ERR_INVALID, "attention: invalid scale %g", (double)scale);
     const spt_tensor none{};
     const spt_tensor &sk = sinks ? *sinks : none;
     if ((rc = validate_bias(&sk, heads, 1))) return rc;

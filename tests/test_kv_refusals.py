@@ -258,3 +258,14 @@ def test_sinks_are_not_written(ctx, what):
     assert c.attend(ctx) == spt.ERR_DEVICE
     c.sinks.data = getattr(c, what) + 32
     assert c.attend(ctx) == spt.ERR_INVALID
+
+
+def test_scales_up_to_the_largest(ctx):
+    """The scale is taken times log2 e in fp32: refused where that is infinite."""
+    import spt
+
+    c = Call()
+    c.scale = 2.3e38
+    assert c.attend(ctx) == spt.ERR_DEVICE
+    c.scale = 2.4e38
+    assert c.attend(ctx) == spt.ERR_INVALID
