@@ -406,7 +406,8 @@ int spt_kv_load_batch(struct spt_ctx *ctx, const spt_kv_cache *cache, const spt_
  * spt_mul_q40_batch_q8_into.  out must not overlap q.
  * work_dev: a workspace of spt_attention_work_bytes bytes, 16-byte aligned, or
  * NULL: the context's arena.  With a workspace the call allocates nothing, so
- * it may be captured into a graph; give each graph and each stream its own.
+ * it may be captured into a graph (without one, and where one is needed, a
+ * captured call is refused); give each graph and each stream its own.
  * Results do not depend on which is used, nor change from call to call. */
 int spt_attention_batch_into(struct spt_ctx *ctx, const spt_kv_cache *cache, const spt_kv_batch *batch,
                              const spt_tensor *sinks, float scale, int32_t window, const float *q_dev,

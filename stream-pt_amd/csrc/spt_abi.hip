@@ -1892,7 +1892,14 @@ int spt_attention_batch_into(spt_ctx *ctx, const spt_kv_cache *cache, const spt_
     if ((rc = check_device(ctx)) || (rc = check_cancel(ctx))) return rc;
     if (batch->n_seqs == 0 || batch->n_rows == 0) return SPT_OK;
     char *work = static_cast<char *>(work_dev);
-    if (!work && call.work_bytes && (rc = arena(ctx, call.work_bytes, &work))) return rc;
+    if (!work && call.work_bytes) {
+        // the arena moves when a later call needs more of it
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        SPT_HIP(hipStreamIsCapturing(ctx->stream, &capture));
+        if (capture != hipStreamCaptureStatusNone)
+            return fail(SPT_ERR_INVALID, "attention: a captured call needs a workspace of %llu bytes of its own", (unsigned long long)call.work_bytes);
+        if ((rc = arena(ctx, call.work_bytes, &work))) return rc;
+    }
     call.a.q = q_dev;
     call.a.out = out_dev;
     call.a.q8 = (uint8_t *)q8_dev;

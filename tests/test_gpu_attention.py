@@ -448,6 +448,40 @@ def test_in_a_graph(new, lens):
         ctx.close()
 
 
+def test_a_captured_call_without_a_workspace():
+    """Refused where it needs one (the arena may move before a replay), and
+    the capture goes on; taken where it needs none."""
+    import torch
+
+    import spt
+
+    stream = torch.cuda.Stream()
+    ctx = spt.Context(0, stream.cuda_stream)
+    try:
+        with torch.cuda.stream(stream):
+            p, short = (Filled(ctx, 4, 2, 64, 32, [1], [n], seed=n) for n in (9000, 50))
+            q = _cuda(p.rng.standard_normal((1, 16, 64)).astype(np.float32))
+            assert ctx.attention_work_bytes(p.cache, p.batch, 16) > 0 == ctx.attention_work_bytes(short.cache, short.batch, 16)
+            out, eager = torch.full_like(q, 9.0), torch.empty_like(q)
+            ctx.attention_batch_into(p.cache, p.batch, q, eager, 0.125)  # the arena is large enough
+            ctx.attention_batch_into(short.cache, short.batch, q, eager, 0.125)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                with pytest.raises(spt.SptError) as e:
+                    ctx.attention_batch_into(p.cache, p.batch, q, out, 0.125)
+                assert e.value.code == spt.ERR_INVALID
+                ctx.attention_batch_into(short.cache, short.batch, q, out, 0.125)
+            for _ in range(3):
+                out.fill_(9.0)
+                graph.replay()
+                stream.synchronize()
+                assert torch.equal(out, eager)
+            del graph
+    finally:
+        ctx.close()
+
+
 def test_two_contexts_at_once():
     """Calls on two streams at once, each with its own context's arena."""
     import torch
