@@ -855,22 +855,24 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
 #pragma unroll
             for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&lds.o[wave][col][32 * b + 16 * h + 4 * g]) = o[c][b][h] * f;
         lds_barrier();
+        // the output's row of this lane's column, to be had from lane r for row r
+        const int fr = row0 + 16 * c + col;
+        const int64_t place = part < 0 ? (int64_t)(sq.r0 + fr / a.group) * a.heads + kvh * a.group + fr % a.group : at + col;
+        float *const outs = part < 0 ? a.out : w.outs;
         constexpr int kQuads = kDim / 4;
-#pragma unroll 4
-        for (int u = lane; u < 16 * kQuads; u += 64) {
-            const int r = u / kQuads, d = u % kQuads * 4, fr = row0 + 16 * c + r;
-            if (16 * c + r >= rows) continue;
-            float *to = part < 0 ? a.out + ((int64_t)(sq.r0 + fr / a.group) * a.heads + kvh * a.group + fr % a.group) * kDim : w.outs + (at + r) * kDim;
-            *reinterpret_cast<f32x4 *>(to + d) = *reinterpret_cast<const f32x4 *>(&lds.o[wave][r][d]);
+#pragma unroll
+        for (int i = 0; i < 16 * kQuads; i += 64) {
+            const int u = i + lane, r = u / kQuads, d = u % kQuads * 4;
+            const int64_t to = __shfl(place, r);
+            if (16 * c + r < rows) *reinterpret_cast<f32x4 *>(outs + to * kDim + d) = *reinterpret_cast<const f32x4 *>(&lds.o[wave][r][d]);
         }
         if (a.q8 && part < 0) {
             for (int u = lane >> 5; u < 16 * NB; u += 2) {
-                const int r = u / NB, b = u % NB, fr = row0 + 16 * c + r;
+                const int r = u / NB, b = u % NB;
                 uint16_t dh;
                 const int x = q8_quantize_half(lds.o[wave][r][32 * b + (lane & 31)], lane, &dh);
-                if (16 * c + r < rows)
-                    write_q8_lane(x, dh, lane & 31, (size_t)(((sq.r0 + fr / a.group) * (int64_t)a.heads + kvh * a.group + fr % a.group) * NB + b),
-                                  nullptr, nullptr, nullptr, a.q8);
+                const int64_t to = __shfl(place, r);
+                if (16 * c + r < rows) write_q8_lane(x, dh, lane & 31, (size_t)(to * NB + b), nullptr, nullptr, nullptr, a.q8);
             }
         }
         lds_barrier();
