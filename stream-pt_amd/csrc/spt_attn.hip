@@ -26,7 +26,7 @@
 // and the MFMAs, which overlap with them in part only (16 MFMAs and 64 FMAs of
 // two waves on a SIMD, one wave each: 463 cycles, 319 and 322 alone).  One
 // token over 1,048,576 positions of 8 heads of 64 (604 MB) takes 144 us, 4.2 TB/s;
-// over 131,071, 28 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times that
+// over 131,071, 27 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times that
 // with the halves): 110 us; of 8,192, 1.31 ms (1,040 TFLOP/s of MFMA).
 #include <algorithm>
 #include <climits>
@@ -52,12 +52,19 @@ constexpr int kWaves = 8;  // of a workgroup (few rows)
 //   up to 4,000: 75, 103; 128 tokens of 32 up to 2,000: 265, 220); more, 128 at a time,
 //   except where 16 at a time are at most a workgroup a compute unit and kChunkTiles
 //   tiles long.
-//   Few rows: a workgroup a unit (a row tile of a sequence and head) up to kDirectTiles
-//   position tiles, and further, up to kWideTiles, in proportion to the units while they
-//   do not fill the compute units (a token of 1 sequence of 2,048: 11.5, shares
-//   12.8; of 4,096: 18.3, 13.2; of 64 ragged ones up to 4,096: 31, 40; up to 16,384:
-//   104, 97); beyond, equal shares of all tiles and a second launch.
-constexpr int kFewRows = 512, kChunkTiles = 96, kDirectTiles = 72, kWideTiles = 300;
+//   Few rows, units (a row tile of a sequence and head) for at most half of the compute
+//   units: each cut into equal parts, a workgroup a part and one a compute unit, and a
+//   second launch that joins them; a workgroup a unit where the parts would save fewer
+//   tiles than that costs, about kSplitTiles / nb (1 sequence of 1,000: 8.2 whole, 10.3 in
+//   parts, of 2,000: 11.5, 10.2, of 4,000: 17.9, 11.0; 8 ragged ones up to 6,000: 24.7,
+//   16.4, heads of 128 in Q8_0: 38.3, 22.4).  Where two workgroups fit a compute unit
+//   and parts pass kLongPart tiles: twice as many parts of one sequence (600,000: 82, 88);
+//   of several, shares (4 of 4 tokens up to 32,000: 36.6, parts 42; up to 10,000: 24.4, 20.4).
+//   More units: a workgroup a unit up to kWideTiles position tiles, in proportion to the
+//   units while they do not fill the compute units (a token of 64 ragged sequences up to
+//   4,096: 31, shares 40; up to 16,384: 104, 97); beyond, equal shares of all tiles
+//   and a second launch.
+constexpr int kFewRows = 512, kChunkTiles = 96, kSplitTiles = 140, kLongPart = 160, kWideTiles = 300;
 constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup of the shares sums up
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
@@ -637,6 +644,21 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_units(AttnA
     if (u.rows) attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
 }
 
+// A workgroup a part of a unit: split_tiles of its position tiles (all, where
+// it has no more).
+template <int BITS, int NB, int ROWS>
+__global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_parts(AttnArgs a) {
+    __shared__ AttnLds<NB> lds;
+    const int kvh = blockIdx.x % a.kv.kv_heads, x = blockIdx.x / a.kv.kv_heads, rt = x % a.row_tiles, split = x / a.row_tiles, seq = blockIdx.y;
+    const Unit u = unit_of<ROWS>(a, kv_seq(a.kv, seq), rt);
+    const int t0 = u.t_lo + split * a.split_tiles, n = (u.tiles() + a.split_tiles - 1) / a.split_tiles;
+    if (u.rows == 0 || split >= n) return;
+    const int64_t unit = ((int64_t)seq * a.row_tiles + rt) * a.kv.kv_heads + kvh, first = unit * (a.splits - 1);
+    // the part of number x is at x + unit
+    if (split == 0 && threadIdx.x == 0) attn_work(a).units[unit] = n == 1 ? make_int2(0, 0) : make_int2((int)first, (int)first + n - 1);
+    attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, t0, min(u.t_hi, t0 + a.split_tiles), n == 1 ? -1 : first + unit + split, lds);
+}
+
 // Rows many at a time: a workgroup's 4 waves have 32 rows each (two columns of
 // the MFMA), and share the tiles' operands, made once a workgroup in LDS: key
 // codes, and values as hi and lo.  While one tile is taken from one buffer, the
@@ -1057,6 +1079,10 @@ __global__ __launch_bounds__(kMergeThreads) void k_attn_merge(AttnArgs a, int ro
 
 }  // namespace
 
+static uint64_t work_bytes(int64_t units, const AttnPlan &p, int nb) {
+    return (uint64_t)(units + 1) / 2 * 16 + (uint64_t)(units + p.groups) * p.unit_rows * (8 + 128 * nb);
+}
+
 AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int max_len, int window, int n_cu) {
     AttnPlan p{};
     const int64_t rows = (int64_t)max_new * group;
@@ -1078,21 +1104,31 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
     const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
     // workgroups at once
     const int64_t resident = (int64_t)n_cu * 4 * (many || nb == 4 ? 2 : kMinWaves<2>) / (many ? kManyWaves : kWaves);
+    const int64_t cost = many ? kManyCost : kUnitCost;
+    const bool long_parts = tiles * units > (int64_t)kLongPart * n_cu && resident > n_cu;
+    if (!many && 2 * units <= n_cu && !(long_parts && n_seqs > 1)) {
+        const int64_t splits = std::min<int64_t>((long_parts ? resident : n_cu) / units, tiles / kWaves);
+        if (splits < 2 || tiles * (splits - 1) * nb <= kSplitTiles * splits) return p;
+        p.split_tiles = (int)((tiles + splits - 1) / splits);
+        p.splits = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
+        p.groups = (int)(units * (p.splits - 1));
+        p.work_bytes = work_bytes(units, p, nb);
+        return p;
+    }
     // 128 rows at a time, us: 1.25 a tile one workgroup a unit, about 18 and 2 a tile of a
     // workgroup's share in shares (768 tokens 39, 65; 128 over 8,192: 320, 80)
-    const bool direct = many ? 5 * tiles * resident <= 72 * resident + 8 * units * tiles : rows > kFewRows || tiles <= std::max<int64_t>(kDirectTiles, std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu));
-    const int64_t cost = many ? kManyCost : kUnitCost;
+    const bool direct = many ? 5 * tiles * resident <= 72 * resident + 8 * units * tiles : rows > kFewRows || tiles <= std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu);
     // (the shares' sums are 32 bits, their merge a workgroup a unit at least)
     if (!direct && entries <= kAttnEntries && units <= (1 << 18) && entries * (tiles + cost) <= INT_MAX) {
         p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + cost) / cost));
-        p.work_bytes = (uint64_t)(units + 1) / 2 * 16 + (uint64_t)(units + p.groups) * p.unit_rows * (8 + 128 * nb);
+        p.work_bytes = work_bytes(units, p, nb);
     }
     return p;
 }
 
 hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
     const bool many = a.unit_rows == kManyRows;
-    const dim3 grid = a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * a.row_tiles, a.kv.n_seqs);
+    const dim3 grid = a.splits ? dim3(a.kv.kv_heads * a.row_tiles * a.splits, a.kv.n_seqs) : a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * a.row_tiles, a.kv.n_seqs);
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, a); };
     auto pick = [&](auto q4_2, auto q4_4, auto q8_2, auto q8_4) {
         if (bits == 4)
@@ -1101,7 +1137,9 @@ hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
             nb == 2 ? go(q8_2) : go(q8_4);
     };
 #define SPT_PICK(kernel, ...) pick(kernel<4, 2, ##__VA_ARGS__>, kernel<4, 4, ##__VA_ARGS__>, kernel<8, 2, ##__VA_ARGS__>, kernel<8, 4, ##__VA_ARGS__>)
-    if (a.groups)
+    if (a.splits)
+        a.unit_rows == 8 ? SPT_PICK(k_attn_parts, 8) : SPT_PICK(k_attn_parts, 16);
+    else if (a.groups)
         many ? SPT_PICK(k_attn_shares, kManyRows) : a.unit_rows == 8 ? SPT_PICK(k_attn_shares, 8) : SPT_PICK(k_attn_shares, 16);
     else
         many ? SPT_PICK(k_attn_many) : a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8) : SPT_PICK(k_attn_units, 16);

@@ -117,6 +117,52 @@ def test_long_sequences(gpu_ctx, bits, dim, kv, group, new, lens, window):
         assert np.array_equal(got, run(gpu_ctx, p, q, dim ** -0.5, window, sk, work=work))
 
 
+@pytest.mark.parametrize("bits,dim,kv,group,new,bound", [
+    (4, 64, 4, 8, 1, 20000), (8, 128, 4, 5, 1, 20000), (4, 128, 2, 8, 3, 9000), (8, 64, 2, 16, 2, 9000), (4, 64, 1, 3, 1, 64000)])
+def test_shares_of_unequal_sequences(gpu_ctx, bits, dim, kv, group, new, bound):
+    """33 sequences, most short or of nothing, for which the bounds allow far more: shares that
+    begin and end in units, whole units, several a share."""
+    lens = [3000, 1700, 0, 640] + [new + 7 * i for i in range(29)]
+    news = [new, new, 0] + [new] * 30
+    p = Filled(gpu_ctx, bits, kv, dim, 32, news, lens, seed=bits)
+    table = np.full((33, -(-bound // 32)), -1, np.int32)
+    table[:, :p.table.shape[1]] = p.table
+    q = p.rng.standard_normal((p.n_rows, kv * group, dim)).astype(np.float32)
+    sk = p.rng.standard_normal(kv * group).astype(np.float32)
+    b = p.make_batch(p.starts, p.lens, new, bound, table=table)
+    assert gpu_ctx.attention_work_bytes(p.cache, b, kv * group) > 0
+    got = run(gpu_ctx, p, q, dim ** -0.5, 0, sk, batch=b)
+    check(got, *p.want(q, dim ** -0.5, 0, sk))
+    for work in (True, False):
+        assert np.array_equal(got, run(gpu_ctx, p, q, dim ** -0.5, 0, sk, batch=b, work=work))
+
+
+@pytest.mark.parametrize("new", (1, 3))
+@pytest.mark.parametrize("bound", (6000, 400000))
+def test_parts_that_cannot_see(gpu_ctx, new, bound):
+    """Sequences cut into parts, by their own and by equal shares: a page that is none in one
+    part makes the row NaN, sequences of nothing and too long ones are as when whole."""
+    lens = [5000, 0, 2600, 40]
+    p = Filled(gpu_ctx, 4, 1, 64, 32, [new, 0, new, new], lens, seed=4)
+    table = np.full((4, -(-bound // 32)), -1, np.int32)
+    table[:, :p.table.shape[1]] = p.table
+    q = p.rng.standard_normal((p.n_rows, 8, 64)).astype(np.float32)
+    want, tol = p.want(q, 0.125)
+    starts = np.array([0, new, 2 * new, 3 * new, 3 * new], np.int32)
+    for page in (0, 80, 5000 // 32):  # the first, one within, the last
+        t = table[[0, 2, 3, 1]].copy()
+        t[0, page] = p.n_pages
+        got = run(gpu_ctx, p, q, 0.125, batch=p.make_batch(starts, [5000, 2600, 40, 0], new, bound, table=t))
+        bad = np.arange(5000 - new, 5000) >= 32 * page
+        assert np.isnan(got[:new][bad]).all()
+        good = np.concatenate([~bad, np.ones(2 * new, bool)])
+        assert (np.abs(got - want) <= tol)[good].all()
+    t = table[[0, 2, 3, 1]]
+    got = run(gpu_ctx, p, q, 0.125, batch=p.make_batch(starts, [bound + 1, -5, 40, bound], new, bound, table=t))
+    assert np.isnan(got[:new]).all() and (got[new:2 * new] == 0).all()
+    assert (np.abs(got - want) <= tol)[2 * new:].all()
+
+
 # Many rows a head, 128 at a time: a workgroup a row tile where there are many, shares of few long ones.
 MANY = [
     (4, 64, 64, 4, [140, 133], [140, 300], 0, True),
