@@ -44,7 +44,8 @@ typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 8;  // of a workgroup (few rows)
+constexpr int kWaves = 8;      // of a workgroup (few rows)
+constexpr int kHalfWaves = 4;  // of one of many
 // Launches, by what the batch's bounds allow (us; heads 64 on 8 of 64, Q4_0):
 //   rows of a key/value head: up to 8, two columns a row (a token of 64 ragged
 //   sequences up to 8,192: 59, a column a row 70); up to kFewRows, 16 at a time (64
@@ -60,7 +61,10 @@ constexpr int kWaves = 8;  // of a workgroup (few rows)
 //   16.4, heads of 128 in Q8_0: 38.3, 22.4).  Where two workgroups fit a compute unit
 //   and parts pass kLongPart tiles: twice as many parts of one sequence (600,000: 82, 88);
 //   of several, shares (4 of 4 tokens up to 32,000: 36.6, parts 42; up to 10,000: 24.4, 20.4).
-//   More units: a workgroup a unit up to kWideTiles position tiles, in proportion to the
+//   More units: a workgroup a unit, of half the waves where units are more than
+//   fit at once (a token of 128 ragged sequences up to 300: 10.6, eight waves 13.7, up to
+//   5,000: 58.9, 59.0; heads of 128, of 34 up to 2,000: 28.5, 34.1, of 64: 29.6, 36.9; of
+//   32, which fit: 20.7, 19.6).  That up to kWideTiles position tiles, in proportion to the
 //   units while they do not fill the compute units (a token of 64 ragged sequences up to
 //   4,096: 31, shares 40; up to 16,384: 104, 97); beyond, equal shares of all tiles
 //   and a second launch.
@@ -423,10 +427,10 @@ struct Query {
     }
 };
 
-template <int NB>
+template <int NB, int WAVES>
 struct AttnLds {
-    float o[kWaves][16][32 * NB + 4];  // by column
-    float m[kWaves][16], l[kWaves][16], sink[16];
+    float o[WAVES][16][32 * NB + 4];  // by column
+    float m[WAVES][16], l[WAVES][16], sink[16];
 };
 
 // The value of lane ^ 8, of each row of 16 lanes.
@@ -445,16 +449,16 @@ __device__ inline half2v other8(half2v x) {
 // the query or the weights and the other by the lo half, which takes a half
 // to two thirds of the MFMAs.  The two lanes add their halves of a score
 // and take half of the tile's positions each through the softmax.
-template <int BITS, int NB, int ROWS>
+template <int BITS, int NB, int ROWS, int WAVES>
 __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, const Unit &un, int seq, int rt, int kvh, int t_begin, int t_end,
-                                                             int64_t part, AttnLds<NB> &lds) {
+                                                             int64_t part, AttnLds<NB, WAVES> &lds) {
     using T = KvTile<BITS, NB>;
     constexpr int kDim = 32 * NB;
     const KvSeq &sq = un.sq;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int t = t_begin + wave;
-    TileWalk walk(a.kv, seq, kvh, t, kWaves, T::kBytes);
+    TileWalk walk(a.kv, seq, kvh, t, WAVES, T::kBytes);
     // Loads are issued on every path: the compiler waits for all of them where
     // paths join.
     auto load = [&](RawTile<BITS, NB> &raw, const TileWalk::Place &p) __attribute__((always_inline)) {
@@ -577,17 +581,17 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
             load(odd, p1);
             const TileWalk::Place p2 = walk.next();
             take(even, p0);
-            t += kWaves;
+            t += WAVES;
             if (t >= t_end) break;
             load(even, p2);
             const TileWalk::Place p3 = walk.next();
             take(odd, p1);
-            t += kWaves;
+            t += WAVES;
             p0 = p2;
             p1 = p3;
         }
     } else {
-        for (; t < t_end; t += kWaves) {
+        for (; t < t_end; t += WAVES) {
             take(even, p0);
             p0 = p1;
             p1 = walk.next();
@@ -603,7 +607,7 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
     __syncthreads();
     float top = lds.m[0][col];
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) top = fmaxf(top, lds.m[w][col]);
+    for (int w = 1; w < WAVES; w++) top = fmaxf(top, lds.m[w][col]);
     const float f = __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
     for (int b = 0; b < NB; b++)
@@ -611,13 +615,13 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
         for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4 *>(&lds.o[wave][col][32 * b + 16 * h + 4 * g]) = o[b][h] * f;
     __syncthreads();
     // a half-wave takes a block of a row
-    for (int u = wave * 2 + (lane >> 5); u < ROWS * NB; u += 2 * kWaves) {
+    for (int u = wave * 2 + (lane >> 5); u < ROWS * NB; u += 2 * WAVES) {
         const int r = u / NB, b = u % NB, d = 32 * b + (lane & 31);
         float mx = lds.m[0][r], sum = 0.0f, den = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, lds.m[w][r]);
+        for (int w = 1; w < WAVES; w++) mx = fmaxf(mx, lds.m[w][r]);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
+        for (int w = 0; w < WAVES; w++) {
             den += lds.l[w][r] * __builtin_amdgcn_exp2f(lds.m[w][r] - mx);
             sum += lds.o[w][r][d];
             if (kPack) sum += lds.o[w][r + 8][d];
@@ -636,19 +640,19 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
 }
 
 // A workgroup a unit.
-template <int BITS, int NB, int ROWS>
-__global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_units(AttnArgs a) {
-    __shared__ AttnLds<NB> lds;
+template <int BITS, int NB, int ROWS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, kMinWaves<NB>) void k_attn_units(AttnArgs a) {
+    __shared__ AttnLds<NB, WAVES> lds;
     const int kvh = blockIdx.x % a.kv.kv_heads, rt = blockIdx.x / a.kv.kv_heads, seq = blockIdx.y;
     const Unit u = unit_of<ROWS>(a, kv_seq(a.kv, seq), rt);
-    if (u.rows) attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
+    if (u.rows) attend<BITS, NB, ROWS, WAVES>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
 }
 
 // A workgroup a part of a unit: split_tiles of its position tiles (all, where
 // it has no more).
 template <int BITS, int NB, int ROWS>
 __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_parts(AttnArgs a) {
-    __shared__ AttnLds<NB> lds;
+    __shared__ AttnLds<NB, kWaves> lds;
     const int kvh = blockIdx.x % a.kv.kv_heads, x = blockIdx.x / a.kv.kv_heads, rt = x % a.row_tiles, split = x / a.row_tiles, seq = blockIdx.y;
     const Unit u = unit_of<ROWS>(a, kv_seq(a.kv, seq), rt);
     const int t0 = u.t_lo + split * a.split_tiles, n = (u.tiles() + a.split_tiles - 1) / a.split_tiles;
@@ -656,7 +660,7 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_parts(AttnA
     const int64_t unit = ((int64_t)seq * a.row_tiles + rt) * a.kv.kv_heads + kvh, first = unit * (a.splits - 1);
     // the part of number x is at x + unit
     if (split == 0 && threadIdx.x == 0) attn_work(a).units[unit] = n == 1 ? make_int2(0, 0) : make_int2((int)first, (int)first + n - 1);
-    attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, t0, min(u.t_hi, t0 + a.split_tiles), n == 1 ? -1 : first + unit + split, lds);
+    attend<BITS, NB, ROWS, kWaves>(a, u, seq, rt, kvh, t0, min(u.t_hi, t0 + a.split_tiles), n == 1 ? -1 : first + unit + split, lds);
 }
 
 // Rows many at a time: a workgroup's 4 waves have 32 rows each (two columns of
@@ -948,7 +952,7 @@ __global__ __launch_bounds__(64 * (ROWS == kManyRows ? kManyWaves : kWaves), ROW
     constexpr bool MANY = ROWS == kManyRows;
     constexpr int kCost = MANY ? kManyCost : kUnitCost;
     constexpr int kGroupWaves = MANY ? kManyWaves : kWaves, kThreads = 64 * kGroupWaves, kEach = kAttnEntries / kThreads;
-    __shared__ std::conditional_t<MANY, ManyLds<NB>, AttnLds<NB>> lds;
+    __shared__ std::conditional_t<MANY, ManyLds<NB>, AttnLds<NB, kWaves>> lds;
     __shared__ int before[kAttnEntries + 1];  // cost of a head before each (sequence, row tile)
     __shared__ int wave_sum[kGroupWaves];
     const int entries = a.kv.n_seqs * a.row_tiles, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1025,7 +1029,7 @@ __global__ __launch_bounds__(64 * (ROWS == kManyRows ? kManyWaves : kWaves), ROW
             if constexpr (MANY)
                 attend_many<BITS, NB>(a, u, seq, rt, kvh, t0, t1, part, lds);
             else
-                attend<BITS, NB, ROWS>(a, u, seq, rt, kvh, t0, t1, part, lds);
+                attend<BITS, NB, ROWS, kWaves>(a, u, seq, rt, kvh, t0, t1, part, lds);
             __syncthreads();
         }
         x = stop;
@@ -1102,6 +1106,7 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
     const bool many = p.unit_rows == kManyRows;
     p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
     const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
+    p.waves = many ? kManyWaves : kWaves;
     // workgroups at once
     const int64_t resident = (int64_t)n_cu * 4 * (many || nb == 4 ? 2 : kMinWaves<2>) / (many ? kManyWaves : kWaves);
     const int64_t cost = many ? kManyCost : kUnitCost;
@@ -1122,6 +1127,8 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
     if (!direct && entries <= kAttnEntries && units <= (1 << 18) && entries * (tiles + cost) <= INT_MAX) {
         p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + cost) / cost));
         p.work_bytes = work_bytes(units, p, nb);
+    } else if (!many && units > resident) {
+        p.waves = kHalfWaves;
     }
     return p;
 }
@@ -1129,7 +1136,7 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
 hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
     const bool many = a.unit_rows == kManyRows;
     const dim3 grid = a.splits ? dim3(a.kv.kv_heads * a.row_tiles * a.splits, a.kv.n_seqs) : a.groups ? dim3(a.groups) : dim3(a.kv.kv_heads * a.row_tiles, a.kv.n_seqs);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * (many ? kManyWaves : kWaves)), 0, s, a); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * a.waves), 0, s, a); };
     auto pick = [&](auto q4_2, auto q4_4, auto q8_2, auto q8_4) {
         if (bits == 4)
             nb == 2 ? go(q4_2) : go(q4_4);
@@ -1141,8 +1148,12 @@ hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
         a.unit_rows == 8 ? SPT_PICK(k_attn_parts, 8) : SPT_PICK(k_attn_parts, 16);
     else if (a.groups)
         many ? SPT_PICK(k_attn_shares, kManyRows) : a.unit_rows == 8 ? SPT_PICK(k_attn_shares, 8) : SPT_PICK(k_attn_shares, 16);
+    else if (many)
+        SPT_PICK(k_attn_many);
+    else if (a.waves == kWaves)
+        a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8, kWaves) : SPT_PICK(k_attn_units, 16, kWaves);
     else
-        many ? SPT_PICK(k_attn_many) : a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8) : SPT_PICK(k_attn_units, 16);
+        a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8, kHalfWaves) : SPT_PICK(k_attn_units, 16, kHalfWaves);
 #undef SPT_PICK
     return hipGetLastError();
 }

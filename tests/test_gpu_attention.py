@@ -137,6 +137,24 @@ def test_shares_of_unequal_sequences(gpu_ctx, bits, dim, kv, group, new, bound):
         assert np.array_equal(got, run(gpu_ctx, p, q, dim ** -0.5, 0, sk, batch=b, work=work))
 
 
+@pytest.mark.parametrize("bits,dim,group,new,window", [(4, 64, 4, 1, 0), (8, 64, 5, 3, 40), (4, 128, 3, 5, 0), (8, 128, 8, 1, 33)])
+def test_more_units_than_fit_at_once(gpu_ctx, bits, dim, group, new, window):
+    """Many heads and sequences: workgroups of fewer waves."""
+    kv = 130
+    p = Filled(gpu_ctx, bits, kv, dim, 32, [new, 0, new, new, new], [new, 40, 33, 161, 70], seed=group, peak=12.0 / np.sqrt(dim), extra_rows=1)
+    q = p.rng.standard_normal((p.n_rows, kv * group, dim)).astype(np.float32)
+    sk = (p.rng.standard_normal(kv * group) * 2).astype(np.float32)
+    got = run(gpu_ctx, p, q, dim ** -0.5, window, sk)
+    check(got, *p.want(q, dim ** -0.5, window, sk))
+    assert (got[-1] == 9.0).all()
+    table = p.table.copy()
+    table[3, 4] = -1  # positions 128 .. 159
+    got2 = run(gpu_ctx, p, q, dim ** -0.5, window, sk, batch=p.make_batch(p.starts, p.lens, new, 161, table=table))
+    bad = np.zeros(p.n_rows, bool)
+    bad[2 * new:3 * new] = True
+    assert np.isnan(got2[bad]).all() and np.array_equal(got2[~bad], got[~bad])
+
+
 @pytest.mark.parametrize("new", (1, 3))
 @pytest.mark.parametrize("bound", (6000, 400000))
 def test_parts_that_cannot_see(gpu_ctx, new, bound):
