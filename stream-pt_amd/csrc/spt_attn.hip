@@ -48,12 +48,8 @@ constexpr int kWaves = 8;      // of a workgroup (few rows)
 constexpr int kHalfWaves = 4;  // of one of many
 // Launches, by what the batch's bounds allow (us; heads 64 on 8 of 64, Q4_0):
 //   rows of a key/value head: up to 8, two columns a row (a token of 64 ragged
-//   sequences up to 8,192: 59, a column a row 70); up to kFewRows, 16 at a time (64
-//   tokens over 16,000 positions: 74, 128 at a time 78; of 8 ragged sequences
-//   up to 4,000: 75, 103; 128 tokens of 32 up to 2,000: 265, 220); more, 128 at a time,
-//   except where 16 at a time are at most a workgroup a compute unit and kChunkTiles
-//   tiles long.
-//   Few rows, units (a row tile of a sequence and head) for at most half of the compute
+//   sequences up to 8,192: 59, a column a row 70); more, 16 or 128 at a time (many_rows).
+//   8 or 16 rows, units (a row tile of a sequence and head) for at most half of the compute
 //   units: each cut into equal parts, a workgroup a part and one a compute unit, and a
 //   second launch that joins them; a workgroup a unit where the parts would save fewer
 //   tiles than that costs, about kSplitTiles / nb (1 sequence of 1,000: 8.2 whole, 10.3 in
@@ -68,7 +64,7 @@ constexpr int kHalfWaves = 4;  // of one of many
 //   units while they do not fill the compute units (a token of 64 ragged sequences up to
 //   4,096: 31, shares 40; up to 16,384: 104, 97); beyond, equal shares of all tiles
 //   and a second launch.
-constexpr int kFewRows = 512, kChunkTiles = 96, kSplitTiles = 140, kLongPart = 160, kWideTiles = 300;
+constexpr int kSplitTiles = 140, kLongPart = 160, kWideTiles = 300;
 constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup of the shares sums up
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
@@ -1087,6 +1083,24 @@ static uint64_t work_bytes(int64_t units, const AttnPlan &p, int nb) {
     return (uint64_t)(units + 1) / 2 * 16 + (uint64_t)(units + p.groups) * p.unit_rows * (8 + 128 * nb);
 }
 
+// Whether 128 rows at a time take less than 16: us of either, for units of `tiles`
+// position tiles at most, of which they have `seen` (without those behind a
+// prompt's own rows, half of them of several sequences, which are rarely all as long
+// as the bounds allow).  Units of 16 rows end evenly; those of 128 last, and where
+// they are few the compute units wait for the longest.  Measured (16 rows at a time, 128;
+// Q4_0, heads of 64): 128 tokens over 2,000 positions 22, 38; a prompt of 1,000: 50, 49,
+// of 2,000: 139, 99; 8 ragged ones up to 100: 18, 13, of 100 tokens over up to 4,000: 103,
+// 194; 32 of 80 over up to 800: 82, 73; window 128, 400 tokens: 17, 14, 200: 11, 15.
+// Q8_0, heads of 128, 200 tokens over 8,000: 112, 125, over 32,000: 604, 384 (tiles
+// behind the caches, and then shares).
+static bool many_rows(int nb, int64_t units16, int64_t units128, int64_t tiles, int64_t own, int n_seqs, int n_cu) {
+    const double seen = double(std::max<int64_t>(1, tiles - own)) * (n_seqs > 1 ? 0.5 : 1.0), slots = 2.0 * n_cu;
+    const bool is_long = nb == 4 && tiles > 256;
+    const double few = 6.0 + (nb == 2 ? 1.0 : is_long ? 2.6 : 2.0) * units16 * (2.0 + 0.2 * seen) / slots;
+    const double scale = nb == 2 ? 1.0 : 1.6, whole = 5.0 + scale * (1.1 * tiles + units128 * (3.0 + 0.6 * seen) / slots);
+    return whole < few || (is_long && 18.0 + scale * 1.9 * seen * units128 / slots < few);
+}
+
 AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int max_len, int window, int n_cu) {
     AttnPlan p{};
     const int64_t rows = (int64_t)max_new * group;
@@ -1097,12 +1111,7 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
         return (window ? std::min<int64_t>(max_len, window + own) : max_len) / kKvTile + 2;
     };
     auto units_of = [&](int unit_rows) { return (int64_t)n_seqs * kv_heads * ((rows + unit_rows - 1) / unit_rows); };
-    if (rows <= 8)
-        p.unit_rows = 8;
-    else if (rows <= kFewRows || (units_of(16) <= n_cu && tiles_of(16) <= kChunkTiles))
-        p.unit_rows = 16;
-    else
-        p.unit_rows = kManyRows;
+    p.unit_rows = rows <= 8 ? 8 : many_rows(nb, units_of(16), units_of(kManyRows), tiles_of(kManyRows), window ? 0 : std::min(max_new, max_len) / 64, n_seqs, n_cu) ? kManyRows : 16;
     const bool many = p.unit_rows == kManyRows;
     p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
     const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
@@ -1121,8 +1130,9 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
         return p;
     }
     // 128 rows at a time, us: 1.25 a tile one workgroup a unit, about 18 and 2 a tile of a
-    // workgroup's share in shares (768 tokens 39, 65; 128 over 8,192: 320, 80)
-    const bool direct = many ? 5 * tiles * resident <= 72 * resident + 8 * units * tiles : rows > kFewRows || tiles <= std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu);
+    // workgroup's share in shares (768 tokens 39, 65; 128 over 8,192: 320, 80); heads of 64
+    // are taken by 16 where shares would be faster
+    const bool direct = many ? nb == 2 || 5 * tiles * resident <= 72 * resident + 8 * units * tiles : tiles <= std::min<int64_t>(kWideTiles, kWideTiles * units / n_cu);
     // (the shares' sums are 32 bits, their merge a workgroup a unit at least)
     if (!direct && entries <= kAttnEntries && units <= (1 << 18) && entries * (tiles + cost) <= INT_MAX) {
         p.groups = (int)std::min<int64_t>(resident, std::max<int64_t>(1, units * (tiles + cost) / cost));
@@ -1147,7 +1157,9 @@ hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
     if (a.splits)
         a.unit_rows == 8 ? SPT_PICK(k_attn_parts, 8) : SPT_PICK(k_attn_parts, 16);
     else if (a.groups)
-        many ? SPT_PICK(k_attn_shares, kManyRows) : a.unit_rows == 8 ? SPT_PICK(k_attn_shares, 8) : SPT_PICK(k_attn_shares, 16);
+        many && bits == 4 ? go(k_attn_shares<4, 4, kManyRows>)  // (only heads of 128 come here)
+        : many            ? go(k_attn_shares<8, 4, kManyRows>)
+        : a.unit_rows == 8 ? SPT_PICK(k_attn_shares, 8) : SPT_PICK(k_attn_shares, 16);
     else if (many)
         SPT_PICK(k_attn_many);
     else if (a.waves == kWaves)

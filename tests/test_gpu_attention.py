@@ -110,7 +110,8 @@ def test_long_sequences(gpu_ctx, bits, dim, kv, group, new, lens, window):
     p = Filled(gpu_ctx, bits, kv, dim, 64, new, lens, seed=3)
     q = p.rng.standard_normal((p.n_rows, kv * group, dim)).astype(np.float32) * 1.5
     sk = p.rng.standard_normal(kv * group).astype(np.float32)
-    assert gpu_ctx.attention_work_bytes(p.cache, p.batch, kv * group, window) > 0
+    # (the last case's row tiles fill the compute units whole)
+    assert (gpu_ctx.attention_work_bytes(p.cache, p.batch, kv * group, window) > 0) == (max(new) < 150)
     got = run(gpu_ctx, p, q, dim ** -0.5, window, sk)
     check(got, *p.want(q, dim ** -0.5, window, sk))
     for work in (True, False):
@@ -135,6 +136,24 @@ def test_shares_of_unequal_sequences(gpu_ctx, bits, dim, kv, group, new, bound):
     check(got, *p.want(q, dim ** -0.5, 0, sk))
     for work in (True, False):
         assert np.array_equal(got, run(gpu_ctx, p, q, dim ** -0.5, 0, sk, batch=b, work=work))
+
+
+@pytest.mark.parametrize("bits,new", [(4, [64]), (8, [3, 64])])
+def test_shares_of_many_rows(gpu_ctx, bits, new):
+    """128 rows at a time of few heads of 128, for which the bounds allow far more positions."""
+    kv, group, bound = 4, 16, 32000
+    lens = [700, 100][:len(new)]
+    p = Filled(gpu_ctx, bits, kv, 128, 32, new, lens, seed=bits, peak=12.0 / np.sqrt(128))
+    table = np.full((len(new), -(-bound // 32)), -1, np.int32)
+    table[:, :p.table.shape[1]] = p.table
+    q = p.rng.standard_normal((p.n_rows, kv * group, 128)).astype(np.float32)
+    sk = p.rng.standard_normal(kv * group).astype(np.float32)
+    b = p.make_batch(p.starts, p.lens, 64, bound, table=table)
+    n = gpu_ctx.attention_work_bytes(p.cache, b, kv * group)
+    assert n > 0
+    got = run(gpu_ctx, p, q, 128 ** -0.5, 0, sk, batch=b)
+    check(got, *p.want(q, 128 ** -0.5, 0, sk))
+    assert np.array_equal(got, run(gpu_ctx, p, q, 128 ** -0.5, 0, sk, batch=b, work=True))
 
 
 @pytest.mark.parametrize("bits,dim,group,new,window", [(4, 64, 4, 1, 0), (8, 64, 5, 3, 40), (4, 128, 3, 5, 0), (8, 128, 8, 1, 33)])
