@@ -23,6 +23,7 @@
 #pragma once
 
 #include "spt_device.h"
+#include "spt_kv_seq.h"
 
 namespace spt {
 
@@ -76,23 +77,8 @@ struct KvArgs {
     const int32_t *pages;
 };
 
-// A sequence of the batch: its rows [r0, r0 + n) (cut to the buffers') and
-// the position of the first; ok: within the batch's declared bounds (else n
-// is cut to them).
-struct KvSeq {
-    int r0, n, len, first;
-    bool ok;
-};
-
 __device__ inline KvSeq kv_seq(const KvArgs &a, int lo, int hi, int len) {
-    KvSeq q;
-    q.r0 = max(0, min(lo, a.n_rows));
-    q.n = max(0, min(hi, a.n_rows) - q.r0);
-    q.len = max(0, len);
-    q.first = q.len - q.n;
-    q.ok = q.len <= a.max_len && q.n <= a.max_new;
-    if (!q.ok) q.n = min(q.n, a.max_new), q.first = 0;
-    return q;
+    return kv_seq_of(lo, hi, len, a.n_rows, a.max_len, a.max_new);
 }
 
 // The batch's arrays, which no kernel here writes, as constant memory: a

@@ -1,0 +1,84 @@
+"""Batches whose arrays claim rows that are not there: nothing behind the
+buffers and no row of no sequence is written, by any of the paths."""
+import numpy as np
+import pytest
+
+from test_gpu_attention import Filled
+from test_gpu_kv_cache import Paged, _cuda
+
+pytestmark = pytest.mark.gpu
+
+LOW, HIGH = -2 ** 31, 2 ** 31 - 1
+
+
+def _starts(n):
+    return [[HIGH, LOW, LOW, HIGH, LOW], [n - 1, LOW, 5, LOW + 5, n], [n, LOW, n - 1, LOW + n - 2, LOW], [0, 5, LOW, 5, LOW + 1],
+            [LOW, HIGH, LOW, HIGH, HIGH], [-5, -2, 1, 0, 40], [30, 20, 10, 5, 2], [LOW, HIGH, -1, HIGH, -7], [HIGH] * 5, [LOW] * 5]
+
+
+def _claimed(starts, n, max_new):
+    rows = np.zeros(n, bool)
+    for lo, hi in zip(starts[:-1], starts[1:]):
+        lo = max(0, lo)
+        rows[lo:max(lo, min(hi, n, lo + max_new))] = True
+    return rows
+
+
+class Guarded:
+    """A buffer of n rows with as many more behind it as a call could reach."""
+
+    def __init__(self, n, behind, row, fill, dtype):
+        import torch
+
+        self.all = torch.full((n + behind, row), fill, dtype=dtype, device="cuda")
+        self.n, self.fill, self.rows = n, fill, self.all[:n]
+
+    def check(self, claimed):
+        got = self.all.cpu().numpy()
+        assert (got[self.n:] == self.fill).all(), "written behind the buffer"
+        assert (got[:self.n][~claimed] == self.fill).all(), "a row of no sequence was written"
+
+
+@pytest.mark.parametrize("bits,dim", [(4, 64), (8, 128)])
+def test_load_and_store(gpu_ctx, bits, dim):
+    import torch
+
+    new, n = 40, 35
+    p = Paged(bits, 2, dim, 32, [new], [90])
+    before = p.data.clone()
+    src = _cuda(p.rng.standard_normal((n, 2 * dim)).astype(np.float32))
+    for starts in _starts(n):
+        for lens in ([8, 8, 8, 8], [HIGH, 0, LOW, 90]):
+            b = p.make_batch(starts, lens, new, 90, n_rows=n, table=np.repeat(p.table, 4, 0))
+            k, v = (Guarded(n, 2 * new, 2 * dim, 7.0, torch.float32) for _ in range(2))
+            gpu_ctx.kv_load_batch(p.cache, b, k.rows, v.rows)
+            k.check(_claimed(starts, n, new))
+            v.check(_claimed(starts, n, new))
+            gpu_ctx.kv_store_batch(p.cache, b, src, src)
+            if all(hi <= lo for lo, hi in zip(starts[:-1], starts[1:])):
+                assert torch.equal(p.data, before)
+            p.data.copy_(before)
+
+
+# rows of a key/value head by 8, by 16 and by 128; whole and in parts
+@pytest.mark.parametrize("bits,dim,kv,group,new,bound", [
+    (4, 64, 1, 2, 4, 100), (4, 64, 1, 2, 4, 9000), (8, 128, 1, 4, 40, 100), (4, 64, 130, 8, 67, 100), (8, 128, 64, 8, 67, 100)])
+def test_attention(gpu_ctx, bits, dim, kv, group, new, bound):
+    import torch
+
+    n = 33
+    p = Filled(gpu_ctx, bits, kv, dim, 32, [new], [90])
+    table = np.full((4, -(-bound // 32)), -1, np.int32)
+    table[:, :p.table.shape[1]] = p.table
+    q = _cuda(p.rng.standard_normal((n, kv * group, dim)).astype(np.float32))
+    row = kv * group * dim
+    for starts in _starts(n):
+        for lens in ([8, 8, 8, 8], [HIGH, 0, LOW, 90]):
+            b = p.make_batch(starts, lens, new, bound, n_rows=n, table=table)
+            out = Guarded(n, 2 * new, row, 9.0, torch.float32)
+            blocks = Guarded(n, 2 * new, row // 32 * 34, 0xAA, torch.uint8)
+            gpu_ctx.attention_batch_into(p.cache, b, q, out.rows, dim ** -0.5, q8=blocks.rows)
+            torch.cuda.synchronize()
+            claimed = _claimed(starts, n, new)
+            out.check(claimed)
+            blocks.check(claimed)
