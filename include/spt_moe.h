@@ -135,12 +135,13 @@ typedef struct spt_kv_cache {
  * in page pages_dev[s * max_pages + p / page_len].  rows_dev, lens_dev and
  * pages_dev are device memory, read by the kernels (a captured graph may be
  * replayed with other lengths and pages in them); the other fields bound them.
- * What they say is not trusted: rows outside the buffers are left out; a row of
- * a position before the first (more rows than positions) is not stored, loads
- * as NaN and attends to nothing; a page outside [0, n_pages) is not stored to,
- * loads as NaN and gives NaN to whoever attends to it; a sequence of more than
- * max_new rows or longer than max_len is not stored, and its first max_new
- * rows load and attend as NaN (its others are left as they were).  Rows
+ * What they say is not trusted: rows outside the buffers are left out (the
+ * others keep their positions); a row of a position before the first (more
+ * rows than positions) is not stored, loads as NaN and attends to nothing; a
+ * page outside [0, n_pages) is not stored to, loads as NaN and gives NaN to
+ * whoever attends to it; a sequence of more than max_new rows or longer than
+ * max_len is not stored, and its first max_new rows of the buffers load and
+ * attend as NaN (its others are left as they were).  Rows
  * that belong to no sequence are left as they were.  No two sequences of a
  * store may share a page that it writes, and no two rows a position; rows that
  * two sequences claim (a rows_dev that falls) hold the results of either.

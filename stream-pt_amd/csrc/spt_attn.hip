@@ -526,7 +526,7 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
                 const int p = mine + j;
                 x[j] = p <= pos && p > from ? x[j] : -__builtin_inff();
             }
-            raw.clear_values(un.p_lo - p0 - 8 * g, sq.len - p0 - 8 * g);
+            raw.clear_values(un.p_lo - p0 - 8 * g, sq.end - p0 - 8 * g);
         }
 #pragma unroll
         for (int j = 0; j < kMine; j++) top = fmaxf(top, x[j]);
@@ -870,11 +870,11 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
             }
     };
 
-    raw.make(oc, lds.buf[0], un.p_lo - t_begin * kKvTile, sq.len - t_begin * kKvTile, wave, lane);
+    raw.make(oc, lds.buf[0], un.p_lo - t_begin * kKvTile, sq.end - t_begin * kKvTile, wave, lane);
     load();
     lds_barrier();
     auto step = [&](int t, int now) __attribute__((always_inline)) {
-        raw.make(oc, lds.buf[now ^ 1], un.p_lo - (t + 1) * kKvTile, sq.len - (t + 1) * kKvTile, wave, lane);
+        raw.make(oc, lds.buf[now ^ 1], un.p_lo - (t + 1) * kKvTile, sq.end - (t + 1) * kKvTile, wave, lane);
         load();
         take(lds.buf[now], t);
         lds_barrier();

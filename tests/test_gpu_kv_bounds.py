@@ -3,8 +3,9 @@ buffers and no row of no sequence is written, by any of the paths."""
 import numpy as np
 import pytest
 
+from kv_reference import attend, stored
 from test_gpu_attention import Filled
-from test_gpu_kv_cache import Paged, _cuda
+from test_gpu_kv_cache import Paged, _cuda, same
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +83,49 @@ def test_attention(gpu_ctx, bits, dim, kv, group, new, bound):
             claimed = _claimed(starts, n, new)
             out.check(claimed)
             blocks.check(claimed)
+
+
+@pytest.mark.parametrize("bits,kv,group,new", [(4, 1, 2, 8), (8, 2, 8, 12), (4, 130, 8, 67)])
+def test_rows_cut_by_the_buffers_keep_their_positions(gpu_ctx, bits, kv, group, new):
+    """The first sequence begins before the buffers, the last ends behind them:
+    their rows that are there are at the positions that they have in whole ones.
+    Positions of the others, never stored, hold marks that no row sees."""
+    import torch
+
+    cut, lens = new // 2, [90, new + 3, 81]
+    p = Paged(bits, kv, 64, 32, [new] * 3, lens, seed=2)
+    p.data.fill_(0xFF)
+    b, starts, n = p.whole()
+    k, v = (p.rng.standard_normal((n, kv, 64)).astype(np.float32) for _ in range(2))
+    # what was in the cache before: all but the new rows of the first and last
+    shifted = [x.copy() for x in (k, v)]
+    for x, y in zip((k, v), shifted):
+        for s in (0, 2):
+            m = lens[s] - new
+            y[starts[s + 1] - m:starts[s + 1]] = x[starts[s]:starts[s] + m]  # last rows are the last positions
+    old = p.make_batch(starts, [lens[0] - new, lens[1], lens[2] - new], 90, 90, n_rows=n)
+    gpu_ctx.kv_store_batch(p.cache, old, _cuda(shifted[0]), _cuda(shifted[1]))
+
+    rows = 3 * new - 2 * cut
+    first, last = -cut, rows + cut  # rows_dev of the batch whose buffers lack cut rows at both ends
+    batch = p.make_batch([first, first + new, first + 2 * new, last], lens, new, 90, n_rows=rows)
+    pick = np.concatenate([np.arange(starts[s + 1] - new, starts[s + 1]) for s in range(3)])[cut:3 * new - cut]
+    gpu_ctx.kv_store_batch(p.cache, batch, _cuda(k[pick]), _cuda(v[pick]))
+    got = p.load(gpu_ctx, batch, rows)
+    want = stored(k, v, bits)
+    assert same(got[0], want[0][pick]) and same(got[1], want[1][pick])
+    whole = p.load(gpu_ctx)
+    there = np.ones(n, bool)
+    there[starts[1] - new:starts[1] - new + cut] = False  # the first sequence's rows before the buffers
+    there[n - cut:] = False
+    assert same(whole[0][there], want[0][there]) and np.isnan(whole[0][~there]).all()
+
+    # attention: the last sequence's rows see nothing that is not there
+    q = p.rng.standard_normal((rows, kv * group, 64)).astype(np.float32)
+    out = torch.full((rows, kv * group, 64), 9.0, device="cuda")
+    gpu_ctx.attention_batch_into(p.cache, batch, _cuda(q), out, 0.125)
+    out = out.cpu().numpy()
+    assert np.isnan(out[:new - cut]).all()  # the first's see the positions before theirs, which are marked
+    for s, a, m in ((1, new - cut, new), (2, 2 * new - cut, new - cut)):
+        w, tol = attend(q[a:a + m], want[0][starts[s]:starts[s + 1]], want[1][starts[s]:starts[s + 1]], lens[s] - new, 0.125)
+        assert (np.abs(out[a:a + m] - w) <= tol).all()

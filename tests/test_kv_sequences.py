@@ -15,7 +15,7 @@ int main() {
     int lo, hi, len, n_rows, max_len, max_new;
     while (scanf("%d %d %d %d %d %d", &lo, &hi, &len, &n_rows, &max_len, &max_new) == 6) {
         const spt::KvSeq q = spt::kv_seq_of(lo, hi, len, n_rows, max_len, max_new);
-        printf("%d %d %d %d %d\n", q.r0, q.n, q.len, q.first, (int)q.ok);
+        printf("%d %d %d %d %d\n", q.r0, q.n, q.first, q.end, (int)q.ok);
     }
 }
 """
@@ -52,9 +52,20 @@ def _cases():
 
 def test_rows_stay_in_the_buffers(sequences):
     """Whatever the arrays hold, rows are inside the buffers and the sequence's."""
-    for (lo, hi, n, rows, max_len, max_new), (r0, got, length, first, ok) in zip(_cases(), sequences(_cases())):
+    for (lo, hi, n, rows, max_len, max_new), (r0, got, _, _, ok) in zip(_cases(), sequences(_cases())):
         what = (lo, hi, n, rows, max_len, max_new)
         assert 0 <= r0 <= rows and 0 <= got <= rows - r0, what
         assert got <= max(0, min(hi, rows) - max(0, lo)) and got <= max_new, what
-        assert length == max(0, n), what
-        assert not ok or length <= max_len, what
+        assert not ok or n <= max_len, what
+
+
+def test_rows_are_the_last_positions(sequences):
+    """Row hi - 1 is the last position, also where rows are cut at either end
+    of the buffers; more rows than declared, cut or not, is a sequence too long."""
+    for (lo, hi, n, rows, max_len, max_new), (r0, got, first, end, ok) in zip(_cases(), sequences(_cases())):
+        what = (lo, hi, n, rows, max_len, max_new)
+        assert ok == (n <= max_len and hi - lo <= max_new), what
+        here = [r for r in (max(lo, 0), min(hi, rows) - 1) if 0 <= r < rows and lo <= r < hi]
+        if ok and here:
+            assert (r0, got) == (here[0], here[-1] - here[0] + 1), what
+            assert [first, end - 1] == [max(0, n) - (hi - r) for r in here], what
