@@ -1883,6 +1883,8 @@ int spt_attention_batch_into(spt_ctx *ctx, const spt_kv_cache *cache, const spt_
     if (ranges_overlap(q8_dev, q8b, q_dev, qb) || ranges_overlap(q8_dev, q8b, out_dev, qb) || ranges_overlap(q8_dev, q8b, cache->data, cache->nbytes) ||
         ranges_overlap(q8_dev, q8b, sk.data, sb) || overlaps_batch(q8_dev, q8b, batch))
         return fail(SPT_ERR_INVALID, "attention: Q8_0 output overlaps an input or the output");
+    // (without rows there is no plan for their heads, and nothing is launched)
+    if (batch->n_seqs == 0 || batch->n_rows == 0) call.work_bytes = 0;
     if (work_dev) {
         if (((uintptr_t)work_dev & 15) || work_bytes < call.work_bytes)
             return fail(SPT_ERR_INVALID, "attention: the workspace must be 16-byte aligned and hold %llu bytes, got %llu",

@@ -269,3 +269,24 @@ def test_scales_up_to_the_largest(ctx):
     assert c.attend(ctx) == spt.ERR_DEVICE
     c.scale = 2.4e38
     assert c.attend(ctx) == spt.ERR_INVALID
+
+
+@pytest.mark.parametrize("empty", ("rows", "sequences"))
+def test_an_empty_batch_needs_no_workspace(ctx, empty):
+    """A workspace sized for the caller's heads is enough for a batch without
+    rows, whose buffers say nothing of the heads; an unaligned one is not."""
+    import spt
+
+    c = Call()
+    c.cache = spt.KVCache.make(spt.TYPE_Q4_0, 8, 64, 64, 5, 1 << 44)
+    c.batch.n_seqs, c.batch.max_new, c.batch.max_len, c.batch.max_pages = 4, 16, 4000, 63
+    n = ctx.attention_work_bytes(c.cache, c.batch, 64)
+    assert n < ctx.attention_work_bytes(c.cache, c.batch, 8)
+    c.work, c.work_bytes = 0x40000000, max(16, n)
+    if empty == "rows":
+        c.batch.n_rows = c.q_len = c.out_len = 0
+    else:
+        c.batch.n_seqs, c.q_len, c.out_len = 0, 7 * 8 * 64, 7 * 8 * 64
+    assert c.attend(ctx) == spt.ERR_DEVICE
+    c.work += 8
+    assert c.attend(ctx) == spt.ERR_INVALID
