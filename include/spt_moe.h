@@ -220,13 +220,18 @@ enum {
     SPT_KERNEL_DOWN_GEMM = 8,    /* grouped down GEMM (large groups)          */
     SPT_KERNEL_Q80 = 9,      /* Q8_0 LM head (GEMV or argmax)                 */
     SPT_KERNEL_RMSNORM = 10, /* RMSNorm (+ Q8_0 of its output)                */
+    SPT_KERNEL_KINDS = 11,   /* of spt_ctx_read_timing: callers were built
+                                with arrays of this size, it stays            */
     SPT_KERNEL_KV = 11,      /* key/value cache store and load                */
     SPT_KERNEL_ATTENTION = 12, /* attention over the cache                    */
-    SPT_KERNEL_KINDS = 13
+    SPT_KERNEL_ALL_KINDS = 13  /* of spt_ctx_read_timing_kinds                */
 };
 int spt_ctx_enable_timing(struct spt_ctx *ctx, int enable);
-/* Synchronise, then write the summed milliseconds and launch counts of each
- * kind since the last read (arrays of SPT_KERNEL_KINDS) and reset them. */
+/* Synchronise, then write the summed milliseconds and launch counts of the
+ * first n_kinds kinds since the last read (arrays of n_kinds, at most
+ * SPT_KERNEL_ALL_KINDS) and reset all kinds. */
+int spt_ctx_read_timing_kinds(struct spt_ctx *ctx, double *total_ms, int64_t *launches, int32_t n_kinds);
+/* The same of the first SPT_KERNEL_KINDS. */
 int spt_ctx_read_timing(struct spt_ctx *ctx, double *total_ms, int64_t *launches);
 
 /* Bytes the context holds in its grow-only device scratch arena and in its

@@ -35,8 +35,8 @@ struct spt_ctx {
     bool timing = false;
     std::vector<std::pair<int, std::pair<hipEvent_t, hipEvent_t>>> pending;
     std::vector<hipEvent_t> free_events;
-    double total_ms[SPT_KERNEL_KINDS] = {};
-    int64_t launches[SPT_KERNEL_KINDS] = {};
+    double total_ms[SPT_KERNEL_ALL_KINDS] = {};
+    int64_t launches[SPT_KERNEL_ALL_KINDS] = {};
     int32_t gemm_min_group = 0;  // 0: the default policy (kGemmMinGroup)
     int32_t decode_max_selections = 0;  // 0: kDecodeMaxSelections; < 0: decode path off
     int n_cu = 0;                // compute units of the device
@@ -1389,8 +1389,14 @@ int spt_ctx_enable_timing(spt_ctx *ctx, int enable) {
 }
 
 int spt_ctx_read_timing(spt_ctx *ctx, double *total_ms, int64_t *launches) {
+    return spt_ctx_read_timing_kinds(ctx, total_ms, launches, SPT_KERNEL_KINDS);
+}
+
+int spt_ctx_read_timing_kinds(spt_ctx *ctx, double *total_ms, int64_t *launches, int32_t n_kinds) {
     int rc;
-    if ((rc = check_ctx(ctx)) || (rc = check_device(ctx))) return rc;
+    if ((rc = check_ctx(ctx))) return rc;
+    if (n_kinds < 1 || n_kinds > SPT_KERNEL_ALL_KINDS) return fail(SPT_ERR_INVALID, "invalid number of kernel kinds: %d", n_kinds);
+    if ((rc = check_device(ctx))) return rc;
     if (!total_ms || !launches) return fail(SPT_ERR_INVALID, "nil output pointer");
     SPT_HIP(hipStreamSynchronize(ctx->stream));
     for (auto &p : ctx->pending) {
@@ -1402,9 +1408,11 @@ int spt_ctx_read_timing(spt_ctx *ctx, double *total_ms, int64_t *launches) {
         ctx->free_events.push_back(p.second.second);
     }
     ctx->pending.clear();
-    for (int k = 0; k < SPT_KERNEL_KINDS; k++) {
-        total_ms[k] = ctx->total_ms[k];
-        launches[k] = ctx->launches[k];
+    for (int k = 0; k < SPT_KERNEL_ALL_KINDS; k++) {
+        if (k < n_kinds) {
+            total_ms[k] = ctx->total_ms[k];
+            launches[k] = ctx->launches[k];
+        }
         ctx->total_ms[k] = 0.0;
         ctx->launches[k] = 0;
     }

@@ -29,7 +29,7 @@ EXPORTED = (
     "spt_mul_q40_batch_into_host", "spt_mul_mxfp4_expert", "spt_route_moe_batch",
     "spt_forward_moe", "spt_forward_moe_batch", "spt_forward_moe_batch_ex",
     "spt_forward_moe_batch_host", "spt_block_sums", "spt_synth_mxfp4",
-    "spt_ctx_enable_timing", "spt_ctx_read_timing", "spt_ctx_set_gemm_min_group",
+    "spt_ctx_enable_timing", "spt_ctx_read_timing", "spt_ctx_read_timing_kinds", "spt_ctx_set_gemm_min_group",
     "spt_mul_q80_into", "spt_mul_q80_argmax", "spt_mul_q80_into_host", "spt_mul_q80_argmax_host",
     "spt_rmsnorm_into", "spt_rmsnorm_batch_into", "spt_mul_q40_batch_bias_into",
     "spt_mul_q40_batch_q8_into", "spt_mul_q40_qkv_batch_into", "spt_forward_moe_batch_q8",
@@ -193,6 +193,7 @@ def lib():
         "spt_synth_mxfp4": ([vp, vp, u64, u64, u64, i32, i32], C.c_int),
         "spt_ctx_enable_timing": ([vp, C.c_int], C.c_int),
         "spt_ctx_read_timing": ([vp, C.POINTER(C.c_double), C.POINTER(C.c_int64)], C.c_int),
+        "spt_ctx_read_timing_kinds": ([vp, C.POINTER(C.c_double), C.POINTER(C.c_int64), i32], C.c_int),
         "spt_upload_range": ([vp, C.c_char_p, u64, u64, T], C.c_int),
         "spt_kv_cache_bytes": ([C.c_uint32, i32, i32, i32, i64, C.POINTER(u64)], C.c_int),
         "spt_kv_store_batch": ([vp, C.POINTER(KVCache), C.POINTER(KVBatch), C.POINTER(Rope), vp, i64, vp, i64, vp, i64, vp, i64],
@@ -286,7 +287,7 @@ class Context:
         """{kind: (total_ms, launches)} since the last read."""
         ms = (C.c_double * len(KERNEL_KINDS))()
         n = (C.c_int64 * len(KERNEL_KINDS))()
-        _check(lib().spt_ctx_read_timing(self.handle, ms, n))
+        _check(lib().spt_ctx_read_timing_kinds(self.handle, ms, n, len(KERNEL_KINDS)))
         return {k: (ms[i], n[i]) for i, k in enumerate(KERNEL_KINDS)}
 
     def memory(self):
