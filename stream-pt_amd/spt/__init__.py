@@ -102,7 +102,7 @@ class KVCache(C.Structure):
         """data: the device buffer (a tensor of cls.bytes(..) bytes, kept
         on the descriptor, or an address)."""
         n = cls.bytes(typ, kv_heads, head_dim, page_len, n_pages)
-        if hasattr(data, "element_size") and data.numel() * data.element_size() < n:
+        if _nbytes(data, n) < n:
             raise ValueError(f"a key/value cache of {n} bytes does not fit the buffer")
         c = cls(typ, kv_heads, head_dim, page_len, n_pages, n, _ptr(data))
         c._keep = data
@@ -229,6 +229,16 @@ def _numel(t):
     if hasattr(t, "numel") and callable(t.numel):
         return int(t.numel())
     return int(t.size)
+
+
+def _nbytes(t, unknown):
+    """Bytes that a tensor in C order holds (unknown: of an address).  A view
+    with strides is none: its elements say nothing of the memory behind it."""
+    if t is None or not hasattr(t, "element_size"):
+        return unknown
+    if not t.is_contiguous():
+        raise ValueError("expected a contiguous tensor")
+    return t.numel() * t.element_size()
 
 
 def _f32(t):
@@ -415,8 +425,13 @@ class Context:
         attention_work_bytes, else the context's arena."""
         nq, pq = _f32(q)
         no, po = _f32(out)
+        blocks = nq // 32 * 34
+        if _nbytes(q8, blocks) < blocks:
+            raise ValueError(f"{blocks} bytes of Q8_0 blocks do not fit the buffer")
+        size = 0 if work is None else _nbytes(work, -1)
+        size = _numel(work) if size < 0 else size
         _check(lib().spt_attention_batch_into(self.handle, _ref(cache), _ref(batch), _ref(sinks), scale, window, pq, nq, po, no,
-                                              _ptr(q8), _ptr(work), _numel(work) if work is not None else 0))
+                                              _ptr(q8), _ptr(work), size))
 
     def mul_mxfp4_expert(self, w: Tensor, bias, expert: int, x, y, batch: int):
         b = bias if bias is not None else Tensor.absent()

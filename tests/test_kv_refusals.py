@@ -290,3 +290,36 @@ def test_an_empty_batch_needs_no_workspace(ctx, empty):
     assert c.attend(ctx) == spt.ERR_DEVICE
     c.work += 8
     assert c.attend(ctx) == spt.ERR_INVALID
+
+
+def test_views_do_not_pass_for_buffers(ctx):
+    """One element expanded, a strided view and too few blocks have as many
+    elements as a buffer, or are taken for one; none has the memory."""
+    import torch
+
+    import spt
+
+    u8 = dict(dtype=torch.uint8)
+    n = spt.KVCache.bytes(spt.TYPE_Q4_0, 2, 64, 64, 5)
+    spt.KVCache.make(spt.TYPE_Q4_0, 2, 64, 64, 5, torch.zeros(n, **u8))
+    for bad in (torch.zeros(1, **u8).expand(n), torch.zeros(2 * n, **u8)[::2], torch.zeros(n - 1, **u8)):
+        with pytest.raises(ValueError):
+            spt.KVCache.make(spt.TYPE_Q4_0, 2, 64, 64, 5, bad)
+    c = Call()
+    c.cache = spt.KVCache.make(spt.TYPE_Q4_0, 2, 64, 64, 5, 1 << 44)
+    c.batch.max_pages, c.batch.max_len = 4096, 200000
+    q, out = torch.zeros(7, 6, 64), torch.zeros(7, 6, 64)
+    blocks, size = q.numel() // 32 * 34, ctx.attention_work_bytes(c.cache, c.batch, 6)
+    attend = lambda **kw: ctx.attention_batch_into(c.cache, c.batch, q, out, 0.125, **kw)  # noqa: E731
+    assert size % 4 == 0
+    for good in (dict(q8=torch.zeros(blocks, **u8)), dict(work=torch.zeros(size, **u8)), dict(work=torch.zeros(size // 4))):
+        with pytest.raises(spt.SptError) as e:
+            attend(**good)
+        assert e.value.code == spt.ERR_DEVICE
+    for bad in (dict(q8=torch.zeros(blocks - 1, **u8)), dict(q8=torch.zeros(1, **u8).expand(blocks)),
+                dict(work=torch.zeros(1, **u8).expand(size)), dict(work=torch.zeros(2 * size, **u8)[::2])):
+        with pytest.raises(ValueError):
+            attend(**bad)
+    with pytest.raises(spt.SptError) as e:
+        attend(work=torch.zeros(size // 4 - 1))
+    assert e.value.code == spt.ERR_INVALID
