@@ -1329,6 +1329,7 @@ int attn_setup(spt_ctx *ctx, const spt_kv_cache *c, const spt_kv_batch *b, int64
     call->a.row_tiles = p.row_tiles;
     call->a.groups = p.groups;
     call->a.waves = p.waves;
+    call->a.chunks = p.chunks;
     call->a.splits = p.splits;
     call->a.split_tiles = p.split_tiles;
     call->work_bytes = p.work_bytes;

@@ -22,6 +22,20 @@
 // kSlack (weights up to 2^kSlack fit fp16 beside the lift), so most tiles need
 // no exchange between lanes and no rescaling.
 //
+// Long rows: fp32 sums of thousands of terms lose small ones behind a large one (one
+// position 2^24 above 131,071 even others: 1.9e-3 of the output, nearly all of it in the
+// sum of the weights), the MFMA cuts each product at 2^-26 of the sum that it is
+// added to, and a weight below 2^-25 is 0 in fp16.  So a wave sums up at most 32 tiles
+// (few rows, kept in LDS) or 64 (many, kept in the output's rows: LDS has no place
+// beside the operands) with a maximum of their own, and joins these sums in fp32;
+// a tile's weights are added in pairs.  Off by at most 7e-6 of sum p |v| there and for other
+// gaps up to 2^32 (2,000 to 131,077 positions, values of one sign; evenly weighted ones
+// 1e-6).  Price: none for few rows (32, 64 tiles: 51.6; as one sum 51.2, 64 ragged tokens up to 8,192);
+// for many none up to 64 tiles, which have kernels without the joins, beyond
+// 1.6 % (a prompt of 8,192: 1,360, 1,338) to 7 % (heads of 128, 4,096 tokens over 8,192: 1,480,
+// 1,386).  A tile's sum made from 0 and added took 13 % more and was off by
+// 4e-6.
+//
 // What bounds it: the vector instructions that unpack values and form weights,
 // and the MFMAs, which overlap with them in part only (16 MFMAs and 64 FMAs of
 // two waves on a SIMD, one wave each: 463 cycles, 319 and 322 alone).  One
@@ -68,7 +82,9 @@ constexpr int kSplitTiles = 140, kLongPart = 160, kWideTiles = 300;
 constexpr int kAttnEntries = 1024;  // (sequence, row tile)s that a workgroup of the shares sums up
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
-constexpr float kLift = 5.0f;       // weights are held times 2^kLift (at most 2^13)
+constexpr float kLift = 7.0f;       // weights are held times 2^kLift (at most 2^15)
+// Position tiles that a wave sums up together (few rows, many).
+constexpr int kFewChunk = 32, kManyChunk = 64;
 
 union Half8 {
     half8v v;
@@ -503,8 +519,9 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
             for (int b = 0; b < NB; b++) {
                 Half8 c;
                 raw.keys(oc, h, b, c);
-                f32x4 s = mfma(c, q.hi[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 if (!kPack) s = mfma(c, q.lo[b], s);
+                s = mfma(c, q.hi[b], s);
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[4 * h + i] = raw.scaled(s[i], h, i, b, b ? x[4 * h + i] : oc.zero);
             }
@@ -543,13 +560,14 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
         }
         Half8 ph, pl;
         const float back = kLift - m;
+        float sums[kMine / 2];
 #pragma unroll
         for (int j = 0; j < kMine; j += 2) {
             const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], q.mul, back)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j + 1], q.mul, back));
-            l += w0;
-            l += w1;
+            sums[j >> 1] = w0 + w1;
             split_pair(oc, w0, w1, ph.h[j >> 1], pl.h[j >> 1]);
         }
+        l += kPack ? sums[0] + sums[1] : (sums[0] + sums[1]) + (sums[kMine / 2 - 2] + sums[kMine / 2 - 1]);
         if (kPack) {
             // the hi column's weights of all positions, and the lo column's
 #pragma unroll
@@ -570,10 +588,45 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
                 o[b][h] = mfma(vl, ph, o[b][h]);
             }
     };
+    // What is summed up goes to this wave's place in LDS, and sums and maximum
+    // begin anew.
+    bool kept = false;
+    int left = kFewChunk;
+    auto join = [&]() __attribute__((always_inline)) {
+        if (kPack) l += other8(l);
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (!kept) return;
+        const float top = fmaxf(m, lds.m[wave][col]), f = __builtin_amdgcn_exp2f(m - top), fk = __builtin_amdgcn_exp2f(lds.m[wave][col] - top);
+        m = top;
+        l = l * f + lds.l[wave][col] * fk;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) o[b][h] = o[b][h] * f + *reinterpret_cast<const f32x4 *>(&lds.o[wave][col][32 * b + 16 * h + 4 * g]) * fk;
+    };
+    auto keep = [&]() __attribute__((always_inline)) {
+        asm volatile("");  // a branch
+        join();
+        // (every lane reads back what it wrote itself)
+        lds.m[wave][col] = m, lds.l[wave][col] = l;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                *reinterpret_cast<f32x4 *>(&lds.o[wave][col][32 * b + 16 * h + 4 * g]) = o[b][h];
+                o[b][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        m = kNoMax, l = 0.0f;
+        kept = true;
+        left = kFewChunk;
+    };
     if (kAhead<BITS, NB, ROWS>) {
         // two tiles in registers, one being loaded while the other is taken
         RawTile<BITS, NB> odd;
         while (t < t_end) {
+            if (left <= 0) keep();
+            left -= 2;
             load(odd, p1);
             const TileWalk::Place p2 = walk.next();
             take(even, p0);
@@ -588,6 +641,8 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
         }
     } else {
         for (; t < t_end; t += WAVES) {
+            if (left == 0) keep();
+            left--;
             take(even, p0);
             p0 = p1;
             p1 = walk.next();
@@ -596,9 +651,7 @@ __device__ __attribute__((always_inline)) inline void attend(const AttnArgs &a, 
     }
 
     // the waves' parts, on the largest maximum
-    if (kPack) l += other8(l);
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    join();
     if (g == 0) lds.m[wave][col] = m, lds.l[wave][col] = l, lds.sink[col] = sink;
     __syncthreads();
     float top = lds.m[0][col];
@@ -668,16 +721,27 @@ __global__ __launch_bounds__(64 * kWaves, kMinWaves<NB>) void k_attn_parts(AttnA
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 
 template <int NB>
-union ManyLds {
+struct ManyLds {
     struct Buffer {
         Half8 k[2 * NB][64];     // [t][b][lane]
         Half8 v[2 * NB][2][64];  // [b][h][hi, lo][lane]
         u32x4 ks[4 * NB];        // scales as they are stored
-    } buf[2];
-    float o[kManyWaves][16][32 * NB + 4];
+    };
+    union {
+        Buffer buf[2];
+        float o[kManyWaves][16][32 * NB + 4];
+    };
+    float2 kept[2][kManyWaves][16];  // maximum and sum of what is kept
 };
 
-// A wave's part of a tile: NB / 2 units of keys (waves 0 to 3) or values.
+// Whether the batch's rows fall somewhere: only then can a row be two sequences'.
+__device__ inline bool rows_fall(const KvArgs &a) {
+    int fall = 0;
+    for (int s = threadIdx.x; s < a.n_seqs; s += 64 * kManyWaves) fall |= a.rows[s + 1] < a.rows[s];
+    return __syncthreads_or(fall) != 0;
+}
+
+// A wave's part of a tile: NB units of keys (waves 0 and 1) or values (2 and 3).
 template <int BITS, int NB>
 struct ManyPart {
     static constexpr int kHalf = kManyWaves / 2, kUnits = 2 * NB / kHalf;  // waves for keys, units of each
@@ -743,7 +807,7 @@ struct ManyPart {
     }
 };
 
-template <int BITS, int NB>
+template <int BITS, int NB, bool CHUNKS>
 __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs &a, const Unit &un, int seq, int rt, int kvh, int t_begin,
                                                                   int t_end, int64_t part, ManyLds<NB> &lds) {
     using T = KvTile<BITS, NB>;
@@ -751,6 +815,10 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
     const KvSeq &sq = un.sq;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // tiles that are summed up together: all of them where another sequence may
+    // claim the rows too, which then hold one of the two results and no mixture
+    int chunk = kManyChunk;
+    if (CHUNKS && part < 0 && t_end - t_begin > kManyChunk && rows_fall(a.kv)) chunk = INT_MAX - 1;
     TileRun run(a.kv, seq, kvh, t_begin, T::kBytes);
     ManyPart<BITS, NB> raw;
     auto load = [&]() __attribute__((always_inline)) {
@@ -804,8 +872,8 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
                 const Half8 k = buf.k[h * NB + b][lane];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    f32x4 s = mfma(k, q[c].hi[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                    s = mfma(k, q[c].lo[b], s);
+                    f32x4 s = mfma(k, q[c].lo[b], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                    s = mfma(k, q[c].hi[b], s);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int n = (i * 2 + h) * NB + b;
@@ -847,14 +915,15 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
 #pragma unroll
         for (int c = 0; c < 2; c++) {
             const float back = kLift - m[c];
+            float sums[4];
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][j], q[c].mul, back));
                 const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][j + 1], q[c].mul, back));
-                l[c] += w0;
-                l[c] += w1;
+                sums[j >> 1] = w0 + w1;
                 split_pair(oc, w0, w1, ph[c].h[j >> 1], pl[c].h[j >> 1]);
             }
+            l[c] += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         }
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -870,6 +939,52 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
             }
     };
 
+    // What is summed up goes to the row's own place in the output (the part's, in
+    // the workspace), and sums and maximum begin anew: registers and LDS hold no
+    // second output.  (Opaque: the loop would carry what the address takes.)
+    bool kept = false;
+    auto kept_at = [&](int c) __attribute__((always_inline)) {
+        int first = row0;
+        asm volatile("" : "+s"(first));
+        const int fr = first + 16 * c + col;
+        const int64_t place = part < 0 ? (int64_t)(sq.r0 + fr / a.group) * a.heads + kvh * a.group + fr % a.group : part * kManyRows + fr - rt * kManyRows;
+        return (part < 0 ? a.out : attn_work(a).outs) + place * kDim + 4 * g;
+    };
+    auto join = [&](int c) __attribute__((always_inline)) {
+        l[c] += __shfl_xor(l[c], 16);
+        l[c] += __shfl_xor(l[c], 32);
+        if (!kept) return;
+        const float2 was = lds.kept[c][wave][col];
+        const float top = fmaxf(m[c], was.x), f = __builtin_amdgcn_exp2f(m[c] - top), fk = __builtin_amdgcn_exp2f(was.x - top);
+        m[c] = top;
+        l[c] = l[c] * f + was.y * fk;
+        const float *from = kept_at(c);
+        if (16 * c + col < rows) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) o[c][b][h] = o[c][b][h] * f + *reinterpret_cast<const f32x4 *>(from + 32 * b + 16 * h) * fk;
+        }
+    };
+    auto keep = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            join(c);
+            // (every lane reads back what it wrote itself)
+            lds.kept[c][wave][col] = make_float2(m[c], l[c]);
+            float *to = kept_at(c);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (16 * c + col < rows) *reinterpret_cast<f32x4 *>(to + 32 * b + 16 * h) = o[c][b][h];
+                    o[c][b][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            m[c] = kNoMax, l[c] = 0.0f;
+        }
+        kept = true;
+    };
+
     raw.make(oc, lds.buf[0], un.p_lo - t_begin * kKvTile, sq.end - t_begin * kKvTile, wave, lane);
     load();
     lds_barrier();
@@ -879,15 +994,19 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
         take(lds.buf[now], t);
         lds_barrier();
     };
-    for (int t = t_begin; t < t_end; t += 2) {
+    for (int t = t_begin, left = chunk; t < t_end; t += 2, left -= 2) {
+        if (CHUNKS && left == 0) {
+            asm volatile("");  // a branch
+            keep();
+            left = chunk;
+        }
         step(t, 0);
         if (t + 1 < t_end) step(t + 1, 1);
     }
 
 #pragma unroll
     for (int c = 0; c < 2; c++) {
-        l[c] += __shfl_xor(l[c], 16);
-        l[c] += __shfl_xor(l[c], 32);
+        join(c);
         m[c] -= kLift;  // weights are 2^kLift too large, the sink is not
         const AttnWork w = attn_work(a);
         const int64_t at = part * kManyRows + wave * 32 + 16 * c;  // the part's rows
@@ -925,15 +1044,15 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
 
 // A workgroup a unit, the last row tiles first: the causal ones with the most
 // tiles, so that the short ones even out the end.
-template <int BITS, int NB>
-__global__ __launch_bounds__(64 * kManyWaves, 2) void k_attn_many(AttnArgs a) {
+template <int BITS, int NB, bool CHUNKS>
+__global__ __launch_bounds__(64 * kManyWaves, NB == 2 ? 3 : 2) void k_attn_many(AttnArgs a) {
     __shared__ ManyLds<NB> lds;
     const int kvh = blockIdx.x % a.kv.kv_heads, seq = blockIdx.y;
     const KvSeq sq = kv_seq(a.kv, seq);
     const int rt = (sq.n * a.group + kManyRows - 1) / kManyRows - 1 - (int)(blockIdx.x / a.kv.kv_heads);
     if (rt < 0) return;
     const Unit u = unit_of<kManyRows>(a, sq, rt);
-    attend_many<BITS, NB>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
+    attend_many<BITS, NB, CHUNKS>(a, u, seq, rt, kvh, u.t_lo, u.t_hi, -1, lds);
 }
 
 // All units' tiles in a row, cut into equal shares, one a workgroup: however
@@ -1023,7 +1142,7 @@ __global__ __launch_bounds__(64 * (ROWS == kManyRows ? kManyWaves : kWaves), ROW
             const int t0 = u.t_lo + (int)(max(x, tile0) - tile0), t1 = min(u.t_hi, u.t_lo + (int)(stop - tile0));
             const int64_t part = alone ? -1 : b + unit;
             if constexpr (MANY)
-                attend_many<BITS, NB>(a, u, seq, rt, kvh, t0, t1, part, lds);
+                attend_many<BITS, NB, true>(a, u, seq, rt, kvh, t0, t1, part, lds);
             else
                 attend<BITS, NB, ROWS, kWaves>(a, u, seq, rt, kvh, t0, t1, part, lds);
             __syncthreads();
@@ -1113,6 +1232,7 @@ AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int
     auto units_of = [&](int unit_rows) { return (int64_t)n_seqs * kv_heads * ((rows + unit_rows - 1) / unit_rows); };
     p.unit_rows = rows <= 8 ? 8 : many_rows(nb, units_of(16), units_of(kManyRows), tiles_of(kManyRows), window ? 0 : std::min(max_new, max_len) / 64, n_seqs, n_cu) ? kManyRows : 16;
     const bool many = p.unit_rows == kManyRows;
+    p.chunks = (window ? tiles_of(p.unit_rows) : (max_len + kKvTile - 1) / kKvTile) > kManyChunk;
     p.row_tiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
     const int64_t entries = (int64_t)n_seqs * p.row_tiles, units = entries * kv_heads, tiles = tiles_of(p.unit_rows);
     p.waves = many ? kManyWaves : kWaves;
@@ -1161,7 +1281,7 @@ hipError_t launch_attn(hipStream_t s, int bits, int nb, const AttnArgs &a) {
         : many            ? go(k_attn_shares<8, 4, kManyRows>)
         : a.unit_rows == 8 ? SPT_PICK(k_attn_shares, 8) : SPT_PICK(k_attn_shares, 16);
     else if (many)
-        SPT_PICK(k_attn_many);
+        a.chunks ? SPT_PICK(k_attn_many, true) : SPT_PICK(k_attn_many, false);
     else if (a.waves == kWaves)
         a.unit_rows == 8 ? SPT_PICK(k_attn_units, 8, kWaves) : SPT_PICK(k_attn_units, 16, kWaves);
     else

@@ -153,6 +153,7 @@ struct AttnArgs {
     int groups;     // parts in the workspace beyond one a unit: of equal shares, their
                     // workgroups; 0: a workgroup a unit, no workspace
     int waves;        // of a workgroup
+    bool chunks;      // 128 rows at a time: more tiles than are summed up together
     int splits;       // most parts of a unit, a workgroup each; 0: equal shares
     int split_tiles;  // position tiles of such a part
     void *work;
@@ -160,6 +161,7 @@ struct AttnArgs {
 // What a call launches, and the workspace that takes.
 struct AttnPlan {
     int unit_rows, row_tiles, waves, groups, splits, split_tiles;
+    bool chunks;
     uint64_t work_bytes;
 };
 AttnPlan attn_plan(int nb, int kv_heads, int group, int n_seqs, int max_new, int max_len, int window, int n_cu);

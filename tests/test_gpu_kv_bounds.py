@@ -129,3 +129,26 @@ def test_rows_cut_by_the_buffers_keep_their_positions(gpu_ctx, bits, kv, group, 
     for s, a, m in ((1, new - cut, new), (2, 2 * new - cut, new - cut)):
         w, tol = attend(q[a:a + m], want[0][starts[s]:starts[s + 1]], want[1][starts[s]:starts[s + 1]], lens[s] - new, 0.125)
         assert (np.abs(out[a:a + m] - w) <= tol).all()
+
+
+def test_rows_of_two_sequences_are_one_of_them(gpu_ctx):
+    """Long rows that two sequences claim hold the results of either: sums on
+    their way are no mixture, though they are kept in the output."""
+    import torch
+
+    kv, new = 130, 67
+    p = Filled(gpu_ctx, 4, kv, 64, 32, [new, 0, new], [2500, 1, 2300], seed=1)
+    q = _cuda(p.rng.standard_normal((new, kv * 8, 64)).astype(np.float32))
+
+    def run(starts):
+        b = p.make_batch(starts, [2500, 0, 2300], new, 2500, n_rows=new)
+        out = torch.full((new, kv * 8, 64), 9.0, device="cuda")
+        gpu_ctx.attention_batch_into(p.cache, b, q, out, 0.125)
+        torch.cuda.synchronize()
+        return out
+
+    first, last = run([0, new, 0, 0]), run([0, 0, 0, new])
+    both = run([0, new, 0, new])
+    near = lambda a, b: (a - b).abs() <= 1e-5 * b.abs() + 1e-6  # noqa: E731
+    assert bool((near(both, first) | near(both, last)).all())
+    assert not bool(near(first, last).all())
