@@ -119,7 +119,7 @@ class KVBatch(C.Structure):
     def make(cls, rows, lens, pages, n_rows, max_new, max_len):
         """rows [n_seqs + 1], lens [n_seqs], pages [n_seqs][max_pages]."""
         for t in (rows, lens, pages):
-            if t.element_size() != 4 or not t.is_contiguous():
+            if t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous():
                 raise ValueError("rows, lens and pages are contiguous int32 tensors")
         if rows.numel() != lens.numel() + 1 or pages.dim() != 2 or pages.shape[0] != lens.numel():
             raise ValueError("rows, lens and pages are of different numbers of sequences")
@@ -245,7 +245,7 @@ def _f32(t):
     """(elements, address) of an fp32 device tensor in C order; None: (0, None)."""
     if t is None:
         return 0, None
-    if t.element_size() != 4 or not t.is_contiguous():
+    if t.element_size() != 4 or not t.is_floating_point() or not t.is_contiguous():
         raise ValueError("expected a contiguous fp32 tensor")
     return t.numel(), t.data_ptr()
 

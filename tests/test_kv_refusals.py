@@ -323,3 +323,28 @@ def test_views_do_not_pass_for_buffers(ctx):
     with pytest.raises(spt.SptError) as e:
         attend(work=torch.zeros(size // 4 - 1))
     assert e.value.code == spt.ERR_INVALID
+
+
+def test_tensors_of_the_other_four_bytes(ctx):
+    """Rows, lengths and pages in fp32, or queries, keys and values in int32,
+    are as large as what is expected, and nothing like it."""
+    import torch
+
+    import spt
+
+    rows, lens, pages = (torch.zeros(n, dtype=torch.int32) for n in (3, 2, (2, 4)))
+    for bad in ((rows.float(), lens, pages), (rows, lens.float(), pages), (rows, lens, pages.float())):
+        with pytest.raises(ValueError):
+            spt.KVBatch.make(*bad, 1, 1, 1)
+    c = Call()
+    kv, q = torch.zeros(7, 2, 64), torch.zeros(7, 6, 64)
+    calls = (lambda x, y: ctx.kv_load_batch(c.cache, c.batch, x, y), lambda x, y: ctx.kv_store_batch(c.cache, c.batch, x, y),
+             lambda x, y: ctx.attention_batch_into(c.cache, c.batch, x, y, 0.125))
+    for call, one in zip(calls, (kv, kv, q)):
+        other = torch.zeros_like(one)
+        with pytest.raises(spt.SptError) as e:
+            call(one, other)
+        assert e.value.code == spt.ERR_DEVICE
+        for bad in ((one.int(), other), (one, other.int())):
+            with pytest.raises(ValueError):
+                call(*bad)
