@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from kv_reference import attend, stored
-from test_gpu_attention import Filled
+from test_gpu_attention import Filled, run
 from test_gpu_kv_cache import Paged, _cuda, same
 
 pytestmark = pytest.mark.gpu
@@ -140,15 +140,27 @@ def test_rows_of_two_sequences_are_one_of_them(gpu_ctx):
     p = Filled(gpu_ctx, 4, kv, 64, 32, [new, 0, new], [2500, 1, 2300], seed=1)
     q = _cuda(p.rng.standard_normal((new, kv * 8, 64)).astype(np.float32))
 
-    def run(starts):
+    def rows_of(starts):
         b = p.make_batch(starts, [2500, 0, 2300], new, 2500, n_rows=new)
         out = torch.full((new, kv * 8, 64), 9.0, device="cuda")
         gpu_ctx.attention_batch_into(p.cache, b, q, out, 0.125)
         torch.cuda.synchronize()
         return out
 
-    first, last = run([0, new, 0, 0]), run([0, 0, 0, new])
-    both = run([0, new, 0, new])
+    first, last = rows_of([0, new, 0, 0]), rows_of([0, 0, 0, new])
+    both = rows_of([0, new, 0, new])
     near = lambda a, b: (a - b).abs() <= 1e-5 * b.abs() + 1e-6  # noqa: E731
     assert bool((near(both, first) | near(both, last)).all())
     assert not bool(near(first, last).all())
+
+
+@pytest.mark.parametrize("new", (4, 40))
+def test_freed_pages_before_a_window_are_never_looked_at(gpu_ctx, new):
+    """Pages whose positions no row sees are none: rows are as with them."""
+    p = Filled(gpu_ctx, 4, 1, 64, 32, [new, new], [100, 90])
+    q = p.rng.standard_normal((2 * new, 8, 64)).astype(np.float32)
+    table = p.table.copy()
+    table[0, 0], table[1, 0] = -1, p.n_pages  # positions 0 .. 31; rows see 56 on and 46 on at least
+    got = [run(gpu_ctx, p, q, 0.125, 5, batch=p.make_batch(p.starts, p.lens, new, 100, table=t)) for t in (p.table, table)]
+    want, tol = p.want(q, 0.125, 5)
+    assert (np.abs(got[1] - want) <= tol).all() and np.array_equal(*got)
