@@ -407,11 +407,11 @@ int spt_kv_load_batch(struct spt_ctx *ctx, const spt_kv_cache *cache, const spt_
  * exp(sink - top)), p_j = exp(scale * q . k_j - top) over positions j up to the
  * row's own and, with window > 0, fewer than window before it.  sinks: optional
  * F32 / F16 / BF16 [heads]; NULL or unnamed: none.  A row that sees nothing is 0.
- * Queries and weights are held to 22 bits, weights not below 2^-32 of the
- * largest among 2,048 positions; sums are fp32, of at most 2,048 positions and
- * then of these sums.  Outputs are off by up to 1e-6 of sum p |v|, by up to 7e-6
- * where one position's weight is some 2^20 to 2^30 times the others' (measured up to
- * 131,077 positions).  q8_dev: NULL, or
+ * Queries are held to 22 bits, weights to 22 bits or to 2^-32 of the largest
+ * among the up to 2,048 positions that are summed up together, in fp32; these
+ * sums are then joined in fp32.  With values of one sign the output is off by up
+ * to 1e-6 of itself, by up to 7e-6 where one position's weight is 2^20 to 2^30
+ * times the others' (measured up to 131,077 positions).  q8_dev: NULL, or
  * q_len/32 GGML Q8_0 blocks that receive the Q8_0 of out, the input of
  * spt_mul_q40_batch_q8_into.  out must not overlap q.
  * work_dev: a workspace of spt_attention_work_bytes bytes, 16-byte aligned, or

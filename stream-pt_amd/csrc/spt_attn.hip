@@ -38,10 +38,14 @@
 //
 // What bounds it: the vector instructions that unpack values and form weights,
 // and the MFMAs, which overlap with them in part only (16 MFMAs and 64 FMAs of
-// two waves on a SIMD, one wave each: 463 cycles, 319 and 322 alone).  One
-// token over 1,048,576 positions of 8 heads of 64 (604 MB) takes 144 us, 4.2 TB/s;
-// over 131,071, 27 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times that
-// with the halves): 110 us; of 8,192, 1.31 ms (1,040 TFLOP/s of MFMA).
+// two waves on a SIMD, one wave each: 463 cycles, 319 and 322 alone); compute units
+// left idle where units are unequal or few (64 ragged tokens up to 8,192: busy 62 %
+// of the time, vector instructions 48 %).  One token over 1,048,576 positions of 8 heads
+// of 64 (604 MB): 129 us and 5 us to join the parts, 4.5 TB/s, vector instructions 70 %;
+// over 131,071, 22 and 5 us.  A prompt of 2,048 tokens, 64 heads (34 GFLOP, 2.5 times
+// that with the halves): 103 us (the same inputs again and again, 112 with others from
+// pass to pass); of 8,192, 1.41 ms (970 TFLOP/s of MFMA; compute units busy 95 %,
+// vector instructions 69 %, MFMA 41 %).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -74,7 +78,8 @@ constexpr int kHalfWaves = 4;  // of one of many
 //   More units: a workgroup a unit, of half the waves where units are more than
 //   fit at once (a token of 128 ragged sequences up to 300: 10.6, eight waves 13.7, up to
 //   5,000: 58.9, 59.0; heads of 128, of 34 up to 2,000: 28.5, 34.1, of 64: 29.6, 36.9; of
-//   32, which fit: 20.7, 19.6).  That up to kWideTiles position tiles, in proportion to the
+//   32, which fit: 20.7, 19.6; in Q8_0, 17 of 40 heads on 8: up to 4,000 33.9, shares 36.6,
+//   up to 5,003 40.3, 40.6, from where shares are taken).  That up to kWideTiles position tiles, in proportion to the
 //   units while they do not fill the compute units (a token of 64 ragged sequences up to
 //   4,096: 31, shares 40; up to 16,384: 104, 97); beyond, equal shares of all tiles
 //   and a second launch.

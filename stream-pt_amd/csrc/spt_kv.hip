@@ -225,7 +225,8 @@ __global__ __launch_bounds__(256) void k_kv_load(KvLoadArgs a) {
 
 // Few rows are shared by heads among up to kv_heads workgroups, while those
 // are fewer than 16 a compute unit (4,099 rows of 64 query and 8 key/value heads
-// of 64: 40.3 us with two a compute unit and rows by eight, 31 us).
+// of 64, the same inputs again: 40.3 us with two a compute unit and rows by eight, 31 us;
+// inputs that change: 38).
 int kv_store_parts(const KvArgs &a, int n_cu) {
     const int64_t chunks = (int64_t)((a.max_new + kStoreRows - 1) / kStoreRows) * a.n_seqs;
     return (int)std::min<int64_t>(a.kv_heads, std::max<int64_t>(1, 16 * (int64_t)n_cu / chunks));
