@@ -96,3 +96,28 @@ def test_sums_keep_what_is_small(gpu_ctx, bits, dim, kv, group, new, seqs, n, sp
                 at = (far / tol).amax(1).argmax().item()
                 assert bool((far <= tol).all()), f"head of gap {GAPS[at % len(GAPS)]}: off by {float((far / mass)[at].max()):.3g}, {float((far / tol).max()):.3g} of what it may"
     assert far2 <= 1e-10 * want2, f"norm off by {(far2 / want2) ** 0.5:.3g}"
+
+
+@pytest.mark.parametrize("bits,dim,kv,group,new,seqs,n", [
+    (8, 64, 8, 8, 1, 64, 40003), (4, 64, 8, 8, 1, 130, 9001), (8, 64, 8, 8, 2, 64, 40003), (4, 64, 8, 8, 16, 150, 12003), (8, 128, 8, 8, 16, 48, 12003)])
+def test_marks_stay_over_kept_sums(gpu_ctx, bits, dim, kv, group, new, seqs, n):
+    """A page that is none, at the beginning, within and at the end of a row
+    that is summed up in several sums, makes it NaN; other sequences are as before."""
+    import torch
+
+    p = Shared(gpu_ctx, bits, kv, dim, seqs, new, n)
+    q = torch.randn(seqs * new, kv * group, dim, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    whole = torch.full_like(q, 9.0)
+    gpu_ctx.attention_batch_into(p.cache, p.many, q, whole, 0.125)
+    table = np.repeat(p.table, seqs, 0)
+    bad = {0: 0, seqs // 2: p.table.shape[1] // 2, seqs - 1: p.table.shape[1] - 1}
+    for s, page in bad.items():
+        table[s, page] = p.n_pages
+    out = torch.full_like(q, 9.0)
+    gpu_ctx.attention_batch_into(p.cache, p.make_batch(np.arange(seqs + 1) * new, [n] * seqs, new, n, n_rows=seqs * new, table=table), q, out, 0.125)
+    torch.cuda.synchronize()
+    lost = torch.zeros(seqs * new, dtype=torch.bool, device="cuda")
+    for s in bad:
+        lost[s * new:(s + 1) * new] = True
+    assert bool(torch.isfinite(whole).all()) and bool(torch.isnan(out[lost]).all())
+    assert torch.equal(out[~lost], whole[~lost])
