@@ -30,10 +30,10 @@
 // beside the operands) with a maximum of their own, and joins these sums in fp32;
 // a tile's weights are added in pairs.  Off by at most 7e-6 of sum p |v| there and for other
 // gaps up to 2^32 (2,000 to 131,077 positions, values of one sign; evenly weighted ones
-// 1e-6).  Price: none for few rows (32, 64 tiles: 51.6; as one sum 51.2, 64 ragged tokens up to 8,192);
-// for many none up to 64 tiles, which have kernels without the joins, beyond
-// 1.6 % (a prompt of 8,192: 1,360, 1,338) to 7 % (heads of 128, 4,096 tokens over 8,192: 1,480,
-// 1,386).  A tile's sum made from 0 and added took 13 % more and was off by
+// 1e-6).  Price: none for few rows (64 ragged tokens up to 8,192 51.6 us, as one sum
+// 51.2); for many none up to 64 tiles, which have kernels without the joins, beyond
+// 3 % (a prompt of 8,192: 1,386, 1,350) to 7 % (heads of 128, 4,096 tokens over 8,192:
+// 1,479, 1,386).  A tile's sum made from 0 and added took 13 % more and was off by
 // 4e-6.
 //
 // What bounds it: the vector instructions that unpack values and form weights,
@@ -79,7 +79,8 @@ constexpr int kHalfWaves = 4;  // of one of many
 //   fit at once (a token of 128 ragged sequences up to 300: 10.6, eight waves 13.7, up to
 //   5,000: 58.9, 59.0; heads of 128, of 34 up to 2,000: 28.5, 34.1, of 64: 29.6, 36.9; of
 //   32, which fit: 20.7, 19.6; in Q8_0, 17 of 40 heads on 8: up to 4,000 33.9, shares 36.6,
-//   up to 5,003 40.3, 40.6, from where shares are taken).  That up to kWideTiles position tiles, in proportion to the
+//   up to 5,003 40.3, 40.6, and beyond in shares).
+//   That up to kWideTiles position tiles, in proportion to the
 //   units while they do not fill the compute units (a token of 64 ragged sequences up to
 //   4,096: 31, shares 40; up to 16,384: 104, 97); beyond, equal shares of all tiles
 //   and a second launch.
@@ -1048,7 +1049,9 @@ __device__ __attribute__((always_inline)) inline void attend_many(const AttnArgs
 }
 
 // A workgroup a unit, the last row tiles first: the causal ones with the most
-// tiles, so that the short ones even out the end.
+// tiles, so that the short ones even out the end.  Heads of 64 at three waves a
+// SIMD (a prompt of 2,048: 101 us, at two 124).  CHUNKS: rows of more than
+// kManyChunk tiles.
 template <int BITS, int NB, bool CHUNKS>
 __global__ __launch_bounds__(64 * kManyWaves, NB == 2 ? 3 : 2) void k_attn_many(AttnArgs a) {
     __shared__ ManyLds<NB> lds;
